@@ -7,7 +7,9 @@ tests and the benchmark.  torch is used only for device memory and streams.  The
 constructor raises when the CUDA library is missing or no GPU is present.
 """
 import ctypes as C
+import functools
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 SO_PATH = os.environ.get("GLMFLASH_B200_SO") or os.path.join(_HERE, "libglmflash_b200.so")
@@ -84,6 +86,11 @@ SYMBOLS = {
     "glmflash_router_logits": (_I, [_P, _P, _I, _P, _I, _I, _I, _P, _I]),
     "glmflash_topk": (_I, [_P, _P, _I, _I, _I, _P, _P, _I]),
     "glmflash_route": (_I, [_P, _P, _I, _P, _I, _I, _I, _I, _P, _P, _P, _I]),
+    "glmflash_topk_rule_bytes": (_Z, []),
+    "glmflash_topk_by": (_I, [_P, _P, C.c_int64, _P, _I, _I, _I, _P, _Z, _P, _P, _I]),
+    "glmflash_route_by": (_I, [_P, _P, C.c_int64, _P, _P, _I, _I, _I, _I, _P, _Z, _P, _P, _P, _I]),
+    "glmflash_linear_args_bytes": (_Z, []),
+    "glmflash_linear": (_I, [_P, _P, _Z]),
     "glmflash_ep_status": (_P, [_P]),
     "glmflash_ep_set_wait_limit": (_I, [_P, C.c_uint32]),
     "glmflash_ep_set_exchange_bf16": (_I, [_P, _I]),
@@ -275,6 +282,8 @@ def lib():
             f.restype, f.argtypes = res, args
         if L.glmflash_abi_version() != 1 or L.glmflash_config_bytes() != C.sizeof(Config) or \
                 L.glmflash_weights_bytes() != C.sizeof(Weights):
+            raise GlmFlashError("ABI mismatch between the python binding and libglmflash_b200.so")
+        if L.glmflash_topk_rule_bytes() != _RULE.size or L.glmflash_linear_args_bytes() != _LINEAR.size:
             raise GlmFlashError("ABI mismatch between the python binding and libglmflash_b200.so")
         _lib = L
     return _lib
@@ -548,6 +557,154 @@ def route(x, wr, logits, picks, weights, stream=None, pdl=1):
     _check(lib().glmflash_route(_stream_ptr(stream), x.data_ptr(), x.stride(0), wr.data_ptr(), rows, wr.shape[1], E,
                                 picks.shape[1] - 1, logits.data_ptr(), picks.data_ptr(), weights.data_ptr(), pdl))
     return picks, weights
+
+
+SCORES = {"sigmoid": 0, "softmax": 1}
+GROUP_SCORES = {"max": 0, "top2": 1}
+ACTS = {"none": 0, "silu": 1, "gelu": 2, "gelu_tanh": 3, "relu": 4}
+_RULE = struct.Struct("=5if2i")                     # glmflash_topk_rule
+_LINEAR = struct.Struct("=12q8if3i")                # glmflash_linear_args
+
+
+def _require(ok, what):
+    if not ok:
+        raise GlmFlashError(what)
+
+
+def _named(table, name, what):
+    _require(name in table, f"{what} must be one of {', '.join(table)}")
+    return table[name]
+
+
+@functools.lru_cache(maxsize=256)
+def _rule(scores, groups, keep_groups, group_score, renorm, scale):
+    return _RULE.pack(_named(SCORES, scores, "scores"), groups, groups if keep_groups is None else keep_groups,
+                      _named(GROUP_SCORES, group_score, "group_score"), int(bool(renorm)), scale, 0, 0)
+
+
+def _table_args(logits, picks, weights, bias):
+    """Checks of a selection's tensors; (rows, experts, device index)."""
+    torch = _torch()
+    _require(logits.dim() == 2 and picks.dim() == 2 and weights.dim() == 2, "logits, picks and weights must have two dimensions")
+    rows, E = logits.shape
+    dev = logits.get_device()
+    _require(dev == torch._C._cuda_getDevice(), "tensors must be on the current CUDA device")
+    _require(logits.dtype is torch.float32 and picks.dtype is torch.int32 and weights.dtype is torch.float32,
+             "logits and weights must be float32, picks int32")
+    _require(picks.get_device() == dev and weights.get_device() == dev, "tensors must be on one device")
+    _require(picks.shape == weights.shape and picks.shape[0] == rows, "picks and weights must be [rows][topk + 1]")
+    _require(picks.is_contiguous() and weights.is_contiguous(), "picks and weights must be contiguous")
+    if bias is not None:
+        _require(bias.dtype is torch.float32 and bias.dim() == 1 and bias.shape[0] == E and bias.get_device() == dev and
+                 (bias.stride(0) == 1 or E == 1), "bias must be float32 [experts], contiguous, on the same device")
+    return rows, E, dev
+
+
+def topk_by(logits, picks, weights, bias=None, scores="sigmoid", groups=1, keep_groups=None, group_score="max", renorm=True, scale=1.0,
+            stream=None, pdl=1):
+    """Routing table of logits fp32 [rows][E] by a rule (glmflash_topk_by): `scores` "sigmoid" or "softmax", `bias` fp32 [E] added to them
+    for the choice alone, `groups` of neighbouring experts of which the `keep_groups` best by `group_score` ("max" or "top2") stay, weights
+    renormalised or not and times `scale`.  Writes picks int32 / weights fp32 [rows][k + 1] (shared expert last) and returns them."""
+    rows, E, _ = _table_args(logits, picks, weights, bias)
+    _require(logits.stride(1) == 1 or E == 1, "logits must have neighbouring experts side by side")
+    _check(lib().glmflash_topk_by(_stream_ptr(stream), logits.data_ptr(), logits.stride(0) if rows > 1 else E,
+                                  None if bias is None else bias.data_ptr(), rows, E, picks.shape[1] - 1,
+                                  _rule(scores, groups, keep_groups, group_score, renorm, scale), _RULE.size, picks.data_ptr(),
+                                  weights.data_ptr(), pdl))
+    return picks, weights
+
+
+def route_by(x, wr, logits, picks, weights, bias=None, scores="sigmoid", groups=1, keep_groups=None, group_score="max", renorm=True,
+             scale=1.0, stream=None, pdl=1):
+    """router_logits + topk_by: x bf16 [rows][hidden], wr bf16 [E][hidden]; fills logits, picks and weights."""
+    torch = _torch()
+    rows, E, dev = _table_args(logits, picks, weights, bias)
+    _require(logits.is_contiguous(), "logits must be contiguous")
+    _require(x.dim() == 2 and wr.dim() == 2 and x.shape[0] == rows and wr.shape[0] == E and x.shape[1] == wr.shape[1],
+             "x must be [rows][hidden] and the router matrix [experts][hidden]")
+    _require(x.dtype is torch.bfloat16 and wr.dtype is torch.bfloat16, "x and the router matrix must be bfloat16")
+    _require(x.get_device() == dev and wr.get_device() == dev, "tensors must be on one device")
+    _require(x.stride(1) == 1 and wr.is_contiguous(), "rows of x and the router matrix must be contiguous")
+    _check(lib().glmflash_route_by(_stream_ptr(stream), x.data_ptr(), x.stride(0) if rows > 1 else x.shape[1], wr.data_ptr(),
+                                   None if bias is None else bias.data_ptr(), rows, wr.shape[1], E, picks.shape[1] - 1,
+                                   _rule(scores, groups, keep_groups, group_score, renorm, scale), _RULE.size, logits.data_ptr(),
+                                   picks.data_ptr(), weights.data_ptr(), pdl))
+    return picks, weights
+
+
+_TYPE_CODES = {}
+
+
+def _type_codes():
+    if not _TYPE_CODES:
+        torch = _torch()
+        _TYPE_CODES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+    return _TYPE_CODES
+
+
+def _dense(x, w, w_up, out, bias, bias_up, act, residual, out_dtype, limit, stream, pdl):
+    torch = _torch()
+    codes, dt, dev = _type_codes(), x.dtype, x.get_device()
+    _require(dev == torch._C._cuda_getDevice(), "tensors must be on the current CUDA device")
+    _require(x.dim() == 2 and w.dim() == 2 and x.shape[1] == w.shape[1], "x must be [rows][inner] and the weights [outer][inner]")
+    rows, K = x.shape
+    N = w.shape[0]
+    _require(rows > 0 and K > 0 and N > 0, "rows, inner and outer must be positive")
+    _require(dt is torch.float16 or dt is torch.bfloat16, "x and the weights must be float16 or bfloat16")
+    ws = us = up = 0
+    for m in (w,) if w_up is None else (w, w_up):
+        _require(m.shape == w.shape and m.dtype is dt and m.get_device() == dev, "the weights must have x's type and device and one shape")
+        _require(m.stride(1) == 1 or K == 1, "the weights must have neighbouring inputs side by side")
+    ws = w.stride(0) if N > 1 else -(-K // 8) * 8          # (the stride of a single row is never used)
+    if w_up is not None:
+        us, up = w_up.stride(0) if N > 1 else ws, w_up.data_ptr()
+    _require(x.stride(1) == 1 or K == 1, "x must have the elements of a row side by side")
+    xs = x.stride(0) if rows > 1 else -(-K // 8) * 8
+    if out is None:
+        if stream is None:
+            out = x.new_empty((rows, N), dtype=out_dtype)
+        else:                                              # (memory of the stream that writes it)
+            with torch.cuda.stream(stream):
+                out = x.new_empty((rows, N), dtype=out_dtype)
+    else:
+        _require(out_dtype is None or out_dtype is out.dtype, "out has another type than out_dtype")
+    ot = out.dtype
+    _require(out.shape == (rows, N) and out.get_device() == dev and (out.stride(1) == 1 or N == 1), "out must be [rows][outer] on x's device, a row's elements side by side")
+    _require(ot is dt or ot is torch.float32, "the output must be float32 or of x's type")
+    bt, bp, bu = 0, 0, 0
+    if bias is not None or bias_up is not None:
+        first = bias if bias is not None else bias_up
+        bt = codes.get(first.dtype, -1)
+        for b in (bias, bias_up):
+            _require(b is None or (b.dtype is first.dtype and b.dim() == 1 and b.shape[0] == N and b.get_device() == dev and (b.stride(0) == 1 or N == 1)),
+                     "a bias must be [outer], contiguous, on x's device (both of one type)")
+        _require(first.dtype is dt or bt == 0, "a bias must be float32 or of x's type")
+        bp, bu = 0 if bias is None else bias.data_ptr(), 0 if bias_up is None else bias_up.data_ptr()
+    rt = rp = rs = 0
+    if residual is not None:
+        rt = codes.get(residual.dtype, -1)
+        _require(residual.shape == (rows, N) and residual.get_device() == dev and (residual.stride(1) == 1 or N == 1),
+                 "the residual must be [rows][outer] on x's device, a row's elements side by side")
+        _require(residual.dtype is dt or rt == 0, "the residual must be float32 or of x's type")
+        rp, rs = residual.data_ptr(), residual.stride(0) if rows > 1 else N
+    args = _LINEAR.pack(x.data_ptr(), w.data_ptr(), up, bp, bu, rp, out.data_ptr(), xs, ws, us, rs, out.stride(0) if rows > 1 else N, rows, K, N, codes[dt],
+                        bt, rt, codes[ot], _named(ACTS, act, "act"), limit, pdl, 0, 0)
+    _check(lib().glmflash_linear(_stream_ptr(stream), args, _LINEAR.size))
+    return out
+
+
+def linear(x, w, out=None, bias=None, act="none", residual=None, out_dtype=None, stream=None, pdl=1):
+    """out = act(x . w^T + bias) + residual (glmflash_linear): x fp16 or bf16 [rows][inner], w of its type [outer][inner], bias [outer] and
+    residual [rows][outer] fp32 or of x's type, out fp32 or of x's type (made here if None; it may be the residual itself).  Rows of x and w
+    are 16-byte aligned (strides multiples of 8).  act: "none", "silu", "gelu", "gelu_tanh" or "relu"."""
+    return _dense(x, w, None, out, bias, None, act, residual, out_dtype, 0.0, stream, pdl)
+
+
+def gated_linear(x, w_gate, w_up, out=None, bias_gate=None, bias_up=None, act="silu", limit=0.0, out_dtype=None, stream=None, pdl=1):
+    """out = act(min(x . w_gate^T + bias_gate, limit)) * clamp(x . w_up^T + bias_up, -limit, limit) in one launch (limit 0: none): the first
+    half of a dense expert.  Tensors as in `linear`."""
+    _require(w_up is not None, "w_up is missing")
+    return _dense(x, w_gate, w_up, out, bias_gate, bias_up, act, None, out_dtype, limit, stream, pdl)
 
 
 def rank_sum(gathered, out, stream=None):

@@ -5,6 +5,7 @@
 //   weight = score / sum of the chosen scores; the row's last slot is the shared expert (id E) with weight 1.
 // Selection is done on the logits (sigmoid is monotonic), so it does not depend on the precision of expf.
 #include "common.cuh"
+#include "select.cuh"
 
 namespace gf {
 
@@ -242,6 +243,23 @@ __global__ void __launch_bounds__(256) route_kernel(const __nv_bfloat16 *__restr
     if (cn > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
 
+constexpr int SEL_WARPS = 4;
+__global__ void __launch_bounds__(SEL_WARPS * 32) select_kernel(const float *logits, int64_t stride, const float *bias, int rows, int E, int topk,
+                                                                SelRule rule, int *picks, float *weights) {
+    extern __shared__ double sel_values[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.x * SEL_WARPS + warp;
+    pdl_wait();
+    pdl_launch_dependents();
+    if (r >= rows) return;
+    select_row(logits + r * stride, bias, E, topk, rule, sel_values + (size_t)warp * E, picks + (size_t)r * (topk + 1), weights + (size_t)r * (topk + 1), lane);
+}
+
+static int launch_select(cudaStream_t s, const float *logits, int64_t stride, const float *bias, int rows, int E, int topk, const SelRule &rule, int *picks,
+                         float *weights, bool pdl) {
+    return launch_k(select_kernel, dim3((unsigned)((rows + SEL_WARPS - 1) / SEL_WARPS)), dim3(SEL_WARPS * 32), (size_t)SEL_WARPS * E * sizeof(double), s, pdl,
+                    logits, stride, bias, rows, E, topk, rule, picks, weights);
+}
+
 static int launch_route(cudaStream_t s, const uint16_t *x, int x_stride, const uint16_t *wr, int rows, int H, int E, int topk, float *logits,
                         int *picks, float *weights, bool pdl) {
     static int sms[64] = {};                       // (threads that come here together set the same)
@@ -295,4 +313,44 @@ extern "C" int glmflash_route(void *stream, const uint16_t *x, int x_stride, con
     GF_REQUIRE(x_stride >= hidden && x_stride % 8 == 0, "x_stride must be >= hidden and a multiple of 8");
     GF_REQUIRE(((uintptr_t)x | (uintptr_t)wr) % 16 == 0, "x and the router matrix must be 16-byte aligned");
     return launch_route((cudaStream_t)stream, x, x_stride, wr, rows, hidden, experts, topk, logits, picks, weights, pdl != 0);
+}
+
+extern "C" size_t glmflash_topk_rule_bytes(void) { return sizeof(glmflash_topk_rule); }
+
+// The rule as the kernels take it, after the checks of the call.
+static int check_rule(const glmflash_topk_rule *rule, size_t bytes, int experts, int topk, SelRule *out) {
+    GF_REQUIRE(bytes == sizeof(glmflash_topk_rule), "rule struct size mismatch");
+    GF_REQUIRE(experts > 0 && experts <= 1024, "experts must be in 1..1024");
+    GF_REQUIRE(rule->scores == GLMFLASH_SCORES_SIGMOID || rule->scores == GLMFLASH_SCORES_SOFTMAX, "scores must be sigmoid (0) or softmax (1)");
+    GF_REQUIRE(rule->group_score == GLMFLASH_GROUP_MAX || rule->group_score == GLMFLASH_GROUP_TOP2, "group_score must be max (0) or top2 (1)");
+    GF_REQUIRE(rule->groups >= 1 && rule->groups <= 32 && experts % rule->groups == 0, "groups must be in 1..32 and divide the number of experts");
+    GF_REQUIRE(rule->keep_groups >= 1 && rule->keep_groups <= rule->groups, "keep_groups must be in 1..groups");
+    GF_REQUIRE(topk >= 1 && topk <= 31 && topk <= experts / rule->groups * rule->keep_groups,
+               "topk must be in 1..31 and at most the number of experts in the groups that stay");
+    GF_REQUIRE(rule->scale - rule->scale == 0.f, "scale must be finite");
+    GF_REQUIRE(!rule->reserved[0] && !rule->reserved[1], "reserved fields must be 0");
+    *out = {rule->scores, rule->groups, rule->keep_groups, rule->group_score, rule->renorm != 0, rule->scale};
+    return 0;
+}
+
+extern "C" int glmflash_topk_by(void *stream, const float *logits, int64_t logits_stride, const float *bias, int rows, int experts, int topk,
+                                const glmflash_topk_rule *rule, size_t rule_bytes, int32_t *picks, float *weights, int pdl) {
+    GF_REQUIRE(logits && rule && picks && weights, "null argument");
+    SelRule sel;
+    if (check_rule(rule, rule_bytes, experts, topk, &sel)) return -1;
+    GF_REQUIRE(rows > 0, "rows must be positive");
+    GF_REQUIRE(logits_stride >= experts, "logits_stride must be at least the number of experts");
+    return launch_select((cudaStream_t)stream, logits, logits_stride, bias, rows, experts, topk, sel, picks, weights, pdl != 0);
+}
+
+extern "C" int glmflash_route_by(void *stream, const uint16_t *x, int64_t x_stride, const uint16_t *wr, const float *bias, int rows, int hidden, int experts,
+                                 int topk, const glmflash_topk_rule *rule, size_t rule_bytes, float *logits, int32_t *picks, float *weights, int pdl) {
+    GF_REQUIRE(x && wr && rule && logits && picks && weights, "null argument");
+    SelRule sel;
+    if (check_rule(rule, rule_bytes, experts, topk, &sel)) return -1;
+    GF_REQUIRE(rows > 0 && hidden > 0 && hidden % 8 == 0, "rows positive; hidden a multiple of 8");
+    GF_REQUIRE(x_stride >= hidden && x_stride % 8 == 0 && x_stride <= INT32_MAX, "x_stride must be >= hidden and a multiple of 8");
+    GF_REQUIRE(((uintptr_t)x | (uintptr_t)wr) % 16 == 0, "x and the router matrix must be 16-byte aligned");
+    if (launch_route((cudaStream_t)stream, x, (int)x_stride, wr, rows, hidden, experts, 0, logits, nullptr, nullptr, pdl != 0)) return -1;
+    return launch_select((cudaStream_t)stream, logits, experts, bias, rows, experts, topk, sel, picks, weights, pdl != 0);
 }

@@ -296,6 +296,72 @@ int glmflash_topk(void *stream, const float *logits, int rows, int experts, int 
 int glmflash_route(void *stream, const uint16_t *x, int x_stride, const uint16_t *wr, int rows, int hidden, int experts,
                    int topk, float *logits, int32_t *picks, float *weights, int pdl);
 
+/* ---- selection by a rule ---------------------------------------------------------------------------------------------
+ * The routers of real checkpoints: upstream's selects its top-8 with a score bias and scales the weights by 2.5
+ * (call sites src/moe.rs:77-111; kernels without published source, parity not pinned: what is below is the definition).
+ * For a row of fp32 logits, l = the logit, or -inf where it is NaN:
+ *   s = 1 / (1 + exp(-l))  or  exp(l - max) / sum exp(l - max) over all experts
+ *   c = s + bias (-inf where the bias is NaN); without a bias c = l, whose order is that of the scores
+ *   groups of experts / groups neighbouring ids: a group's value is its largest c, or the sum of its two largest c (without a
+ *     bias: s); the keep_groups largest stay, ties to the lower group
+ *   picks = the topk largest c of the groups that stay, descending, ties to the lower id
+ *   weight = s * scale, or with renorm s / (sum of the chosen s) * scale, 0 where that sum is 0
+ * The order is that of s and c in 64 bits (values that 32 bits cannot tell apart are no tie); weights are computed in fp32 or more.
+ * Every row gets topk different ids in 0..experts-1 and finite weights, whatever its logits: a softmax row whose largest logit
+ * is +inf shares 1 among its infinities, one without a logit above -inf has scores of 0.  A bias of -inf closes an expert as
+ * long as topk others are open.  As in glmflash_topk the last slot names the shared expert (id = experts) with weight 1. */
+typedef struct glmflash_topk_rule {
+    int32_t scores;        /* GLMFLASH_SCORES_*                                                                */
+    int32_t groups;        /* 1..32, divides experts; 1: no groups                                             */
+    int32_t keep_groups;   /* 1..groups; topk <= keep_groups * experts / groups                                */
+    int32_t group_score;   /* GLMFLASH_GROUP_*                                                                 */
+    int32_t renorm;        /* 1: weights of a row sum to scale                                                 */
+    float   scale;         /* finite (upstream 2.5)                                                            */
+    int32_t reserved[2];   /* 0                                                                                */
+} glmflash_topk_rule;
+enum { GLMFLASH_SCORES_SIGMOID = 0, GLMFLASH_SCORES_SOFTMAX = 1 };
+enum { GLMFLASH_GROUP_MAX = 0, GLMFLASH_GROUP_TOP2 = 1 };
+size_t glmflash_topk_rule_bytes(void);
+/* logits fp32 [rows][logits_stride >= experts], bias fp32 [experts] or NULL, experts 1..1024, topk 1..31; picks int32 and weights
+ * fp32 [rows][topk + 1].  rule: host memory, read during the call.  Enqueues work only (graph-capturable); pdl as above. */
+int glmflash_topk_by(void *stream, const float *logits, int64_t logits_stride, const float *bias, int rows, int experts, int topk,
+                     const glmflash_topk_rule *rule, size_t rule_bytes, int32_t *picks, float *weights, int pdl);
+/* The router product (glmflash_router_logits) and the selection from the logits that it leaves in `logits` (fp32 [rows][experts]):
+ * the bytes of the two calls one after the other. */
+int glmflash_route_by(void *stream, const uint16_t *x, int64_t x_stride, const uint16_t *wr, const float *bias, int rows, int hidden,
+                      int experts, int topk, const glmflash_topk_rule *rule, size_t rule_bytes, float *logits, int32_t *picks,
+                      float *weights, int pdl);
+
+/* ---- dense products beside the path ----------------------------------------------------------------------------------
+ * The projections that a checkpoint keeps dense around the expert path: upstream's shared expert (`_fmm`, `_swiglu`, `_fmm`,
+ * src/moe.rs:132-167; FP8 there, fp16 or bf16 weights here), a vocabulary head.
+ *   w_up == NULL   out = act(x . w^T + bias) + residual
+ *   w_up != NULL   out = act(min(g, limit)) * min(max(u, -limit), limit),  g = x . w^T + bias, u = x . w_up^T + bias_up
+ * x [rows][x_stride], weights [outer][stride], of `type`; only the first `inner` elements of a row are read.  Sums and the epilogue
+ * are fp32, the result is rounded once, to out_type.  residual [rows][residual_stride] may be the output itself (same type and
+ * stride); the output may overlap nothing else.  Strides in elements; those of x and the weights multiples of 8, their bases 16-byte
+ * aligned; output and residual of any stride.  NaN and infinities go through as the formula says (a limit does not hide a NaN).
+ * With an owner whose shared_exl3 is 0 the dense shared expert of a layer is the gated form into a buffer and the plain form
+ * with residual = out = glmflash_moe_output.  Enqueues work only, needs no workspace, shares nothing between calls. */
+typedef struct glmflash_linear_args {
+    const void *x, *w, *w_up;                            /* w_up: NULL, or the second matrix of the gated form         */
+    const void *bias, *bias_up, *residual;               /* NULL: none; bias_up with w_up only, residual without       */
+    void       *out;
+    int64_t     x_stride, w_stride, w_up_stride, residual_stride, out_stride;
+    int32_t     rows, inner, outer;                      /* out [rows][outer]; each in 1..2^30                          */
+    int32_t     type;                                    /* GLMFLASH_F16 or GLMFLASH_BF16                               */
+    int32_t     bias_type, residual_type, out_type;      /* GLMFLASH_F32 or `type`                                      */
+    int32_t     act;                                     /* GLMFLASH_ACT_*                                              */
+    float       limit;                                   /* gated form: clamp of upstream's SwiGLU, 0: none             */
+    int32_t     pdl;                                     /* as glmflash_config.pdl                                      */
+    int32_t     reserved[2];                             /* 0                                                           */
+} glmflash_linear_args;
+enum { GLMFLASH_F32 = 0, GLMFLASH_F16 = 1, GLMFLASH_BF16 = 2 };
+/* gelu: v (1 + erf(v / sqrt 2)) / 2;  gelu_tanh: v (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))) / 2 */
+enum { GLMFLASH_ACT_NONE = 0, GLMFLASH_ACT_SILU = 1, GLMFLASH_ACT_GELU = 2, GLMFLASH_ACT_GELU_TANH = 3, GLMFLASH_ACT_RELU = 4 };
+size_t glmflash_linear_args_bytes(void);
+int glmflash_linear(void *stream, const glmflash_linear_args *args, size_t args_bytes);
+
 /* ---- prepared weights  (src/prepared.rs:15-377; layout: docs/ARTIFACTS.md "Prepared target") ---------------------
  * A prepared model is a JSON manifest (format 1: file size, chunk size, one SHA-256 per chunk, storage table, object
  * tree with tensor leaves, preparation key) next to its payload `data.bin`.  open parses and validates the manifest
