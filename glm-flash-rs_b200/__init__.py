@@ -91,6 +91,8 @@ SYMBOLS = {
     "glmflash_route_by": (_I, [_P, _P, C.c_int64, _P, _P, _I, _I, _I, _I, _P, _Z, _P, _P, _P, _I]),
     "glmflash_linear_args_bytes": (_Z, []),
     "glmflash_linear": (_I, [_P, _P, _Z]),
+    "glmflash_linear_status": (_P, []),
+    "glmflash_linear_clear_status": (_I, [_P]),
     "glmflash_ep_status": (_P, [_P]),
     "glmflash_ep_set_wait_limit": (_I, [_P, C.c_uint32]),
     "glmflash_ep_set_exchange_bf16": (_I, [_P, _I]),
@@ -705,6 +707,16 @@ def gated_linear(x, w_gate, w_up, out=None, bias_gate=None, bias_up=None, act="s
     half of a dense expert.  Tensors as in `linear`."""
     _require(w_up is not None, "w_up is missing")
     return _dense(x, w_gate, w_up, out, bias_gate, bias_up, act, None, out_dtype, limit, stream, pdl)
+
+
+def linear_status():
+    """Status word of `linear` and `gated_linear` on the current device: 0, or non-zero when a bounded wait inside a kernel gave up."""
+    torch = _torch()
+    return _view(lib().glmflash_linear_status(), (1,), torch.int32)
+
+
+def linear_clear_status(stream=None):
+    _check(lib().glmflash_linear_clear_status(_stream_ptr(stream)))
 
 
 def rank_sum(gathered, out, stream=None):

@@ -1,54 +1,9 @@
 // Dense products beside the quantised ones: out = act(x . w^T + bias) + residual and the gated pair
 // out = act(min(x . wg^T + bg, limit)) * clamp(x . wu^T + bu, -limit, limit), fp16 or bf16 operands, fp32 sums, one rounding at the end.
 // The projections around the expert path that a checkpoint keeps dense (the shared expert of an upstream bank, a vocabulary head).
-#include "common.cuh"
+#include "dense.cuh"
 
 namespace gf {
-
-struct DenseArgs {
-    const void *x, *w[2], *bias[2], *residual;
-    void *out;
-    int64_t xs, ws[2], rs, os;
-    int rows, K, N, type, bias_type, residual_type, out_type, act;
-    float limit;                                         // 0: none
-};
-
-__device__ __forceinline__ float dense_load(const void *p, int64_t i, int type) {
-    if (type == GLMFLASH_F32) return static_cast<const float *>(p)[i];
-    return type == GLMFLASH_F16 ? __half2float(static_cast<const __half *>(p)[i]) : __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
-}
-__device__ __forceinline__ void dense_store(void *p, int64_t i, int type, float v) {
-    if (type == GLMFLASH_F32) static_cast<float *>(p)[i] = v;
-    else if (type == GLMFLASH_F16) static_cast<__half *>(p)[i] = __float2half_rn(v);
-    else static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(v);
-}
-__device__ __forceinline__ float dense_act(float v, int act) {
-    switch (act) {
-        case GLMFLASH_ACT_SILU: return silu(v);
-        case GLMFLASH_ACT_GELU: return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
-        case GLMFLASH_ACT_GELU_TANH: return 0.5f * v * (1.f + tanhf(0.79788456080286536f * (v + 0.044715f * v * v * v)));
-        case GLMFLASH_ACT_RELU: return v < 0.f ? 0.f : v;                            // (NaN stays)
-        default: return v;
-    }
-}
-// clamps that let NaN through (fminf and fmaxf would drop it)
-__device__ __forceinline__ float dense_below(float v, float limit) { return v > limit ? limit : v; }
-__device__ __forceinline__ float dense_within(float v, float limit) { return v > limit ? limit : v < -limit ? -limit : v; }
-
-// What follows the sums of output column n of row r.
-template <int MATS>
-__device__ __forceinline__ void dense_finish(const DenseArgs &a, int r, int n, float g, float u) {
-    if (a.bias[0]) g += dense_load(a.bias[0], n, a.bias_type);
-    if (MATS == 2) {
-        if (a.bias[1]) u += dense_load(a.bias[1], n, a.bias_type);
-        if (a.limit > 0.f) { g = dense_below(g, a.limit); u = dense_within(u, a.limit); }
-        g = dense_act(g, a.act) * u;
-    } else {
-        g = dense_act(g, a.act);
-        if (a.residual) g += dense_load(a.residual, r * a.rs + n, a.residual_type);
-    }
-    dense_store(a.out, r * a.os + n, a.out_type, g);
-}
 
 template <bool BF>
 __device__ __forceinline__ void dense_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -174,6 +129,7 @@ extern "C" int glmflash_linear(void *stream, const glmflash_linear_args *p, size
                    p->out_stride, p->rows, p->inner, p->outer, p->type, p->bias_type, p->residual_type, p->out_type, p->act, p->limit};
     const bool bf = p->type == GLMFLASH_BF16, pdl = p->pdl != 0;
     cudaStream_t s = (cudaStream_t)stream;
+    if (p->rows > 64) return dense_wide(s, a, pdl);
     if (gated) return bf ? launch_dense<true, 2>(s, a, pdl) : launch_dense<false, 2>(s, a, pdl);
     return bf ? launch_dense<true, 1>(s, a, pdl) : launch_dense<false, 1>(s, a, pdl);
 }

@@ -361,6 +361,9 @@ enum { GLMFLASH_F32 = 0, GLMFLASH_F16 = 1, GLMFLASH_BF16 = 2 };
 enum { GLMFLASH_ACT_NONE = 0, GLMFLASH_ACT_SILU = 1, GLMFLASH_ACT_GELU = 2, GLMFLASH_ACT_GELU_TANH = 3, GLMFLASH_ACT_RELU = 4 };
 size_t glmflash_linear_args_bytes(void);
 int glmflash_linear(void *stream, const glmflash_linear_args *args, size_t args_bytes);
+/* Device status word of the current device's calls, as glmflash_experts_status, and its reset in stream order. */
+const int32_t *glmflash_linear_status(void);
+int glmflash_linear_clear_status(void *stream);
 
 /* ---- prepared weights  (src/prepared.rs:15-377; layout: docs/ARTIFACTS.md "Prepared target") ---------------------
  * A prepared model is a JSON manifest (format 1: file size, chunk size, one SHA-256 per chunk, storage table, object
