@@ -72,14 +72,15 @@ __global__ void __launch_bounds__(DN_WARPS * 32) dense_kernel(const DenseArgs a,
     if (tid >= 8 * RT * DN_N) return;
     const int r = tid / DN_N, n = tid % DN_N;
     if (r0 + r >= a.rows || n0 + n >= a.N) return;
-    float v[MATS];
+    float v[MATS][1], b[2];
+    dense_biases<MATS>(a, n0 + n, b);
 #pragma unroll
     for (int m = 0; m < MATS; ++m) {
-        v[m] = 0.f;
+        v[m][0] = 0.f;
 #pragma unroll
-        for (int w = 0; w < DN_WARPS; ++w) v[m] += part[w][m][r][n];
+        for (int w = 0; w < DN_WARPS; ++w) v[m][0] += part[w][m][r][n];
     }
-    dense_finish<MATS>(a, r0 + r, n0 + n, v[0], v[MATS - 1]);
+    dense_finish<MATS>(a, r0 + r, n0 + n, 1, v[0], v[MATS - 1], b);
 }
 
 template <bool BF, int MATS>
@@ -129,7 +130,7 @@ extern "C" int glmflash_linear(void *stream, const glmflash_linear_args *p, size
                    p->out_stride, p->rows, p->inner, p->outer, p->type, p->bias_type, p->residual_type, p->out_type, p->act, p->limit};
     const bool bf = p->type == GLMFLASH_BF16, pdl = p->pdl != 0;
     cudaStream_t s = (cudaStream_t)stream;
-    if (p->rows > 64) return dense_wide(s, a, pdl);
+    if (p->rows > 16) return dense_gemm(s, a, pdl);
     if (gated) return bf ? launch_dense<true, 2>(s, a, pdl) : launch_dense<false, 2>(s, a, pdl);
     return bf ? launch_dense<true, 1>(s, a, pdl) : launch_dense<false, 1>(s, a, pdl);
 }

@@ -16,41 +16,55 @@ __device__ __forceinline__ float dense_load(const void *p, int64_t i, int type) 
     if (type == GLMFLASH_F32) return static_cast<const float *>(p)[i];
     return type == GLMFLASH_F16 ? __half2float(static_cast<const __half *>(p)[i]) : __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
 }
-__device__ __forceinline__ void dense_store(void *p, int64_t i, int type, float v) {
-    if (type == GLMFLASH_F32) static_cast<float *>(p)[i] = v;
-    else if (type == GLMFLASH_F16) static_cast<__half *>(p)[i] = __float2half_rn(v);
-    else static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(v);
-}
 __device__ __forceinline__ float dense_gelu(float v) { return 0.5f * v * (1.f + erff(v * 0.70710678118654752f)); }
 __device__ __forceinline__ float dense_gelu_tanh(float v) { return 0.5f * v * (1.f + tanhf(0.79788456080286536f * (v + 0.044715f * v * v * v))); }
-__device__ __forceinline__ float dense_act(float v, int act) {
-    switch (act) {
-        case GLMFLASH_ACT_SILU: return silu(v);
-        case GLMFLASH_ACT_GELU: return dense_gelu(v);
-        case GLMFLASH_ACT_GELU_TANH: return dense_gelu_tanh(v);
-        case GLMFLASH_ACT_RELU: return v < 0.f ? 0.f : v;                            // (NaN stays)
-        default: return v;
-    }
-}
 // clamps that let NaN through (fminf and fmaxf would drop it)
 __device__ __forceinline__ float dense_below(float v, float limit) { return v > limit ? limit : v; }
 __device__ __forceinline__ float dense_within(float v, float limit) { return v > limit ? limit : v < -limit ? -limit : v; }
 
-// What follows the sums of output column n of row r.
-template <int MATS>
-__device__ __forceinline__ void dense_finish(const DenseArgs &a, int r, int n, float g, float u) {
-    if (a.bias[0]) g += dense_load(a.bias[0], n, a.bias_type);
-    if (MATS == 2) {
-        if (a.bias[1]) u += dense_load(a.bias[1], n, a.bias_type);
-        if (a.limit > 0.f) { g = dense_below(g, a.limit); u = dense_within(u, a.limit); }
-        g = dense_act(g, a.act) * u;
-    } else {
-        g = dense_act(g, a.act);
-        if (a.residual) g += dense_load(a.residual, r * a.rs + n, a.residual_type);
+// What follows the sums of output column n of rows r .. r + ROWS - 1, of which the first `count` are there: bias (b), activation and residual, or
+// the gated pair.  Chosen by comparisons around all rows: a jump table in front of every value cost 400 clocks each.
+template <int ROWS, typename F>
+__device__ __forceinline__ void dense_each(F f) {
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) f(i);
+}
+template <int ROWS>
+__device__ __forceinline__ void dense_act(float (&v)[ROWS], int act) {
+    if (act == GLMFLASH_ACT_NONE) return;
+    if (act == GLMFLASH_ACT_SILU) dense_each<ROWS>([&](int i) { v[i] = silu(v[i]); });
+    else if (act == GLMFLASH_ACT_GELU) dense_each<ROWS>([&](int i) { v[i] = dense_gelu(v[i]); });
+    else if (act == GLMFLASH_ACT_GELU_TANH) dense_each<ROWS>([&](int i) { v[i] = dense_gelu_tanh(v[i]); });
+    else dense_each<ROWS>([&](int i) { v[i] = v[i] < 0.f ? 0.f : v[i]; });                                 // (NaN stays)
+}
+template <int MATS, int ROWS>
+__device__ __forceinline__ void dense_finish(const DenseArgs &a, int64_t r, int n, int count, float (&g)[ROWS], float (&u)[ROWS], const float (&b)[2]) {
+    float res[ROWS];
+    if (MATS == 1 && a.residual) {                       // (rows behind the last one read it once more: no branch between the loads)
+        const int64_t at = r * a.rs + n;
+        if (a.residual_type == GLMFLASH_F32) dense_each<ROWS>([&](int i) { res[i] = static_cast<const float *>(a.residual)[at + min(i, count - 1) * a.rs]; });
+        else if (a.residual_type == GLMFLASH_F16) dense_each<ROWS>([&](int i) { res[i] = __half2float(static_cast<const __half *>(a.residual)[at + min(i, count - 1) * a.rs]); });
+        else dense_each<ROWS>([&](int i) { res[i] = __bfloat162float(static_cast<const __nv_bfloat16 *>(a.residual)[at + min(i, count - 1) * a.rs]); });
     }
-    dense_store(a.out, r * a.os + n, a.out_type, g);
+    dense_each<ROWS>([&](int i) { g[i] += b[0]; });
+    if (MATS == 2) {
+        dense_each<ROWS>([&](int i) { u[i] += b[1]; });
+        if (a.limit > 0.f) dense_each<ROWS>([&](int i) { g[i] = dense_below(g[i], a.limit); u[i] = dense_within(u[i], a.limit); });
+    }
+    dense_act(g, a.act);
+    if (MATS == 2) dense_each<ROWS>([&](int i) { g[i] *= u[i]; });
+    else if (a.residual) dense_each<ROWS>([&](int i) { g[i] += res[i]; });
+    const int64_t at = r * a.os + n;
+    if (a.out_type == GLMFLASH_F32) dense_each<ROWS>([&](int i) { if (i < count) static_cast<float *>(a.out)[at + i * a.os] = g[i]; });
+    else if (a.out_type == GLMFLASH_F16) dense_each<ROWS>([&](int i) { if (i < count) static_cast<__half *>(a.out)[at + i * a.os] = __float2half_rn(g[i]); });
+    else dense_each<ROWS>([&](int i) { if (i < count) static_cast<__nv_bfloat16 *>(a.out)[at + i * a.os] = __float2bfloat16_rn(g[i]); });
+}
+template <int MATS>
+__device__ __forceinline__ void dense_biases(const DenseArgs &a, int n, float (&b)[2]) {
+#pragma unroll
+    for (int m = 0; m < 2; ++m) b[m] = m < MATS && a.bias[m] && n < a.N ? dense_load(a.bias[m], n, a.bias_type) : 0.f;
 }
 
-int dense_wide(cudaStream_t s, const DenseArgs &a, bool pdl);
+int dense_gemm(cudaStream_t s, const DenseArgs &a, bool pdl);
 
 }  // namespace gf

@@ -2,15 +2,19 @@
 //
 // The weights are the M operand, the rows N: an output column is a lane of tensor memory, a row a column of it, so that only as many rows
 // are multiplied as there are (in 32).  Pairs of CTAs (cta_group::2, 256 output columns x up to 256 rows), one CTA per SM, walk tiles:
-//   warp 0     copies 128 rows of the weights and half of the tile's rows a stage (64 k), of each CTA
+//   warps 0, 3 copy 128 rows of the weights and half of the tile's rows a stage (128 k), of each CTA
 //   warp 1     (first CTA) issues the products of the pair
 //   warp 2     allocates and frees tensor memory
 //   warps 4-11 epilogue: bias, activation, residual or the gated pair, one rounding, while the next pass is multiplied
 // A tile is one PASS over K into one of two sets of accumulators.  The gated pair is two passes, gate and up, on the same rows; the
 // epilogue keeps act(gate) in registers.  With an fp32 output a pass covers at most 512 k and the epilogue adds passes in fp32 (CHAIN): the
 // tensor core truncates as it accumulates, over 4096 k far beyond what fp32 sums are off by.
+// Stages are 128 k long because a turn of the copying thread (wait, announce, copy) takes 170 ns whatever it copies, and each copy beyond the
+// first 37 (weights and rows have a thread each): with 64 k and two copies a turn an SM took in 80 GB/s, with one CTA alone as with 148, at any depth of the ring; it can take 117
+// (all SMs at once).  Where K is a multiple of 64 one copy brings both halves of a stage.
 // Every wait is bounded; one that gives up sets the status word, every role leaves, copies in flight land, tensor memory is freed.
 #include <algorithm>
+#include <initializer_list>
 
 #include "dense.cuh"
 #include "tcgen05.cuh"
@@ -19,9 +23,10 @@ namespace gf {
 
 __device__ int dense_status_word;
 
-constexpr int DW_STAGES = 6, DW_HALF = 128 * 128, DW_STAGE = 2 * DW_HALF, DW_THREADS = 384, DW_ROWS = 256;
-constexpr int DW_CHAIN = 512 / 64;                           // stages of a pass that is one of several
-constexpr size_t DW_SMEM = 1024 + (size_t)DW_STAGES * DW_STAGE + 256;
+constexpr int DW_K = 128, DW_A = 128 * DW_K * 2;             // k of a stage; bytes of its weights in a CTA
+constexpr int DW_DEPTH = 5, DW_RING = 3 * (DW_A + 256 * 128), DW_THREADS = 384, DW_ROWS = 256;
+constexpr int DW_CHAIN = 512 / DW_K;                         // stages of a pass that is one of several
+constexpr size_t DW_SMEM = 1024 + DW_RING + 256;
 constexpr int DW_REGS_COPY = 40, DW_REGS_EPI = 232;          // launched with 168 x 384: (40 + 2 x 232) x 128
 static_assert(DW_REGS_COPY + 2 * DW_REGS_EPI <= 3 * 168, "registers");
 
@@ -29,7 +34,16 @@ struct DenseMaps { CUtensorMap w[2], x; };
 
 struct DenseTiles {
     int bn, across, tiles, stages, pass;                     // rows of a tile, tiles of 256 output columns, all tiles, stages of K, stages of a pass
+    int depth, copies;                                       // stages of the ring, copies that bring a stage of an operand
 };
+
+// A stage of `rows` rows: two tiles of 64 k one behind the other.  One copy of a [64][rows][2] box, or two of [64][rows] (K is no multiple of
+// 64: the end of a row has to be seen).
+template <typename F>
+__device__ __forceinline__ void dense_copy(unsigned char *dst, int stage, int rows, int copies, F copy) {
+    copy(dst, 2 * stage);
+    if (copies == 2) copy(dst + rows * 128, 2 * stage + 1);
+}
 
 // Values of one lane (output column n, bias b) for 32 rows from r on: what follows the sums, without the store.
 template <int MATS>
@@ -40,25 +54,7 @@ __device__ __forceinline__ void dense_act32(const DenseArgs &a, float (&v)[32], 
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = dense_below(v[i], a.limit);
     }
-    switch (a.act) {
-        case GLMFLASH_ACT_SILU:
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = silu(v[i]);
-            break;
-        case GLMFLASH_ACT_GELU:
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = dense_gelu(v[i]);
-            break;
-        case GLMFLASH_ACT_GELU_TANH:
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = dense_gelu_tanh(v[i]);
-            break;
-        case GLMFLASH_ACT_RELU:
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = v[i] < 0.f ? 0.f : v[i];
-            break;
-        default: break;
-    }
+    dense_act(v, a.act);
 }
 // Walks `count` rows (more than 0) in 32 steps, staying on the last: addresses without a branch between the loads, so that all are on their
 // way at once.
@@ -86,9 +82,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(DW_THREADS, 1)
 dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, const DenseTiles d) {
     extern __shared__ unsigned char smem_raw[];
     unsigned char *ring = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    uint64_t *full = reinterpret_cast<uint64_t *>(ring + (size_t)DW_STAGES * DW_STAGE);   // (first CTA) the copies of both have landed
-    uint64_t *done = full + DW_STAGES;                       // products of the stage done, in both CTAs
-    uint64_t *acc_full = done + DW_STAGES;                   // [2] a pass is complete, in both
+    uint64_t *full = reinterpret_cast<uint64_t *>(ring + DW_RING);        // (first CTA) the copies of both have landed
+    uint64_t *done = full + DW_DEPTH;                        // products of the stage done, in both CTAs
+    uint64_t *acc_full = done + DW_DEPTH;                    // [2] a pass is complete, in both
     uint64_t *acc_empty = acc_full + 2;                      // [2] (first CTA) read by the epilogue warps of both
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_empty + 2);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
@@ -96,7 +92,7 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = (int)t5_cta_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     if (tid == 0) {
-        for (int s = 0; s < DW_STAGES; ++s) { mbar_init(full + s, 1); mbar_init(done + s, 1); }
+        for (int s = 0; s < DW_DEPTH; ++s) { mbar_init(full + s, 2); mbar_init(done + s, 1); }
         for (int b = 0; b < 2; ++b) { mbar_init(acc_full + b, 1); mbar_init(acc_empty + b, 16); }
         *abort_flag = 0;
         mbar_fence_init();
@@ -109,32 +105,36 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
     pdl_wait();
     pdl_launch_dependents();
     const int items = d.tiles > pair ? (d.tiles - pair + pairs - 1) / pairs : 0;
-    const uint32_t stages = (uint32_t)items * MATS * d.stages;
+    const uint32_t stages = (uint32_t)items * MATS * d.stages, depth = d.depth, slot_bytes = DW_A + d.bn * 128;
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(DW_REGS_COPY));
-        if (warp == 0 && lane == 0) {
+        if ((warp == 0 || warp == 3) && lane == 0) {
             const uint32_t full0 = t5_of_cta(full, 0);       // (the copies of both CTAs count on the first one's barrier)
+            const bool rows = warp == 3;
+            const int box = rows ? d.bn >> 1 : 128;
             T5Ring at;
             uint32_t it = 0;
             bool ok = true;
             for (int tile = pair; ok && tile < d.tiles; tile += pairs) {
-                const int n = (tile % d.across) * 256 + rank * 128, r = (tile / d.across) * d.bn + rank * (d.bn >> 1);
-                for (int m = 0; m < MATS && ok; ++m)
+                const int y = rows ? (tile / d.across) * d.bn + rank * box : (tile % d.across) * 256 + rank * 128;
+                for (int m = 0; m < MATS && ok; ++m) {
+                    const CUtensorMap *map = rows ? &maps.x : &maps.w[m];
                     for (int s = 0; s < d.stages; ++s, ++it) {
-                        if (it >= DW_STAGES && !t5_wait<200>(done + at.slot, at.parity ^ 1, abort_flag, status, GF_STATUS_TMA_TIMEOUT)) { ok = false; break; }
-                        if (rank == 0) mbar_expect_tx(full + at.slot, 2u * (DW_HALF + (uint32_t)(d.bn >> 1) * 128));
-                        unsigned char *dst = ring + at.slot * DW_STAGE;
-                        t5_load_pair(dst, &maps.w[m], s * 64, n, full0 + 8 * at.slot);
-                        t5_load_pair(dst + DW_HALF, &maps.x, s * 64, r, full0 + 8 * at.slot);
-                        at.next(DW_STAGES);
+                        if (it >= depth && !t5_wait<200>(done + at.slot, at.parity ^ 1, abort_flag, status, GF_STATUS_TMA_TIMEOUT)) { ok = false; break; }
+                        if (rank == 0) mbar_expect_tx(full + at.slot, 2 * box * DW_K * 2);
+                        const uint32_t bar = full0 + 8 * at.slot;
+                        dense_copy(ring + at.slot * slot_bytes + (rows ? DW_A : 0), s, box, d.copies, [&](unsigned char *to, int k) { t5_load_pair(to, map, d.copies == 1, k, y, bar); });
+                        at.next(depth);
                     }
+                }
             }
             // after a give-up: copies in flight have landed before the CTA leaves (the second CTA's count elsewhere: it stays that long)
             if (!ok || *abort_flag)
-                for (uint32_t k = it > DW_STAGES ? it - DW_STAGES : 0; k < it; ++k) mbar_wait((rank ? done : full) + k % DW_STAGES, (k / DW_STAGES) & 1, nullptr, 1000u);
+                for (uint32_t k = it > depth ? it - depth : 0; k < it; ++k) mbar_wait((rank ? done : full) + k % depth, (k / depth) & 1, nullptr, 1000u);
         } else if (warp == 1 && rank == 0) {
             const uint32_t idesc = t5_idesc(256, d.bn, a.type == GLMFLASH_BF16);
             const uint64_t desc0 = t5_desc(smem_u32(ring));
+            const uint32_t next = d.bn * 64 >> 4;            // from the first 64 k of the rows to the second
             T5Ring at;
             uint32_t pc = 0;
             bool ok = true;
@@ -149,15 +149,16 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
                         ok = __all_sync(0xffffffffu, t5_wait<0>(full + at.slot, at.parity, abort_flag, status, GF_STATUS_MMA_TIMEOUT));
                         if (!ok) break;
                         t5_fence_after();
-                        const uint64_t da = desc0 + at.slot * (DW_STAGE >> 4), db = da + (DW_HALF >> 4);
+                        const uint64_t da = desc0 + at.slot * (slot_bytes >> 4), db = da + (DW_A >> 4);
                         if (t5_elect()) {
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) t5_mma<2>(acc, da + 2 * k, db + 2 * k, idesc, k > 0 || s > 0);
+                            for (int k = 0; k < DW_K / 16; ++k)
+                                t5_mma<2>(acc, da + 2 * (k & 3) + (k >> 2) * (128 * 128 >> 4), db + 2 * (k & 3) + (k >> 2) * next, idesc, k > 0 ? 1u : s > 0);
                             t5_commit<2>(done + at.slot);
                             if (s == end - 1) t5_commit<2>(acc_full + b);
                         }
                         __syncwarp();
-                        at.next(DW_STAGES);
+                        at.next(depth);
                     }
                 }
         }
@@ -257,8 +258,8 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
             }
         }
         // the arrivals of the last commits have come in before this CTA ends
-        for (uint32_t k = stages > DW_STAGES ? stages - DW_STAGES : 0; k < stages && ok; ++k)
-            ok = t5_wait<200>(done + k % DW_STAGES, (k / DW_STAGES) & 1, abort_flag, status, GF_STATUS_MMA_TIMEOUT);
+        for (uint32_t k = stages > depth ? stages - depth : 0; k < stages && ok; ++k)
+            ok = t5_wait<200>(done + k % depth, (k / depth) & 1, abort_flag, status, GF_STATUS_MMA_TIMEOUT);
     }
     t5_fence_before();
     // the pair ends together (not the aligned form: single lanes of warps 0 and 1 worked alone)
@@ -267,51 +268,285 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
     if (warp == 2) t5_dealloc<2>(tmem, 512);
 }
 
-// [rows][stride] of 16-bit elements, boxes of 64 elements x box_rows
-static int dense_map(CUtensorMap *map, const void *base, bool bf, int64_t rows, int K, int64_t stride, int box_rows, const char *what) {
-    const uint64_t dims[2] = {(uint64_t)K, (uint64_t)rows}, strides[1] = {(uint64_t)stride * 2};
-    const uint32_t box[2] = {64, (uint32_t)box_rows};
-    return encode_map(map, bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void *>(base), dims, strides, box, what);
+// ---------------------------------------------------------------------------------------------------------- few tiles
+// Too few tiles for a pair each: single CTAs (128 output columns x up to 256 rows) of a CLUSTER that cuts K between them.  Each multiplies its
+// part, and sends the sums in fours of rows to the CTA of the cluster that finishes them (distributed shared memory, one way, 16 bytes a
+// lane); after a cluster barrier that one adds the parts in ascending order and runs the epilogue.
+//   warps 0, 2 copy weights and rows;  warp 1 allocates tensor memory and issues the products;  warps 4-11 epilogue
+constexpr int DT_THREADS = 384, DT_DEPTH = 8, DT_SMEM = 224 * 1024;
+
+struct DenseThin {
+    int t, row_tiles, stages, chains;                        // rows of a tile (in 16), tiles of rows, stages of K, sums of at most 512 k a CTA
+    int depth, copies, slots, alias, cols;                   // stages of the ring, copies that bring a stage of an operand, fours of rows a CTA finishes, the parts lie over the ring, tensor memory
+};
+
+template <int MATS>
+__global__ void __launch_bounds__(DT_THREADS, 1)
+dense_thin_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, const DenseThin d) {
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char *ring = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    __shared__ uint64_t full[DT_DEPTH], done[DT_DEPTH], acc_full;
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_word;
+    volatile int *abort_flag = &abort_word;
+    int *status = &dense_status_word;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    uint32_t cn;
+    asm("mov.u32 %0, %cluster_nctarank;" : "=r"(cn));
+    const int rank = (int)t5_cta_rank(), tile = blockIdx.x / cn, n0 = tile / d.row_tiles * 128, r0 = tile % d.row_tiles * d.t;
+    const int first = (int)((int64_t)d.stages * rank / cn), mine = (int)((int64_t)d.stages * (rank + 1) / cn) - first;    // stages of this CTA
+    const uint32_t bytes = MATS * DW_A + (uint32_t)d.t * DW_K * 2;
+    float4 *parts = reinterpret_cast<float4 *>(ring + (d.alias ? 0 : (size_t)d.depth * bytes));       // [cn][slots][MATS][128]
+    if (tid == 0) {
+        for (int s = 0; s < d.depth; ++s) { mbar_init(full + s, 2); mbar_init(done + s, 1); }
+        mbar_init(&acc_full, 1);
+        abort_word = 0;
+        mbar_fence_init();
+    }
+    __syncthreads();
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");     // (waited for in front of the first store to a peer)
+    bool ok = true;
+    if (warp == 0 || warp == 2) {                            // (they do not wait for the tensor memory)
+        pdl_wait();
+        if (lane == 0) {
+            T5Ring at;
+            int it = 0;
+            for (; it < mine; ++it) {
+                if (it >= d.depth && !t5_wait<200>(done + at.slot, at.parity ^ 1, abort_flag, status, GF_STATUS_TMA_TIMEOUT)) break;
+                unsigned char *dst = ring + (size_t)at.slot * bytes;
+                mbar_expect_tx(full + at.slot, warp ? d.t * DW_K * 2 : MATS * DW_A);
+                if (warp == 0)
+                    for (int m = 0; m < MATS; ++m)
+                        dense_copy(dst + m * DW_A, first + it, 128, d.copies, [&](unsigned char *to, int k) { t5_load(to, &maps.w[m], d.copies == 1, k, n0, full + at.slot); });
+                else
+                    dense_copy(dst + MATS * DW_A, first + it, d.t, d.copies, [&](unsigned char *to, int k) { t5_load(to, &maps.x, d.copies == 1, k, r0, full + at.slot); });
+                at.next(d.depth);
+            }
+            // after a give-up: copies in flight have landed before the CTA leaves
+            if (it < mine || *abort_flag)
+                for (int k = max(it - d.depth, 0); k < it; ++k) mbar_wait(full + k % d.depth, (k / d.depth) & 1, nullptr, 1000u);
+        }
+    } else if (warp == 1) {
+        // (The next kernel of the stream may start only now: one that took the SM's tensor memory first would wait for this one, which waits for it.)
+        t5_alloc<1>(&tmem_slot, d.cols);
+        pdl_launch_dependents();
+        pdl_wait();
+        t5_fence_before();
+        asm volatile("barrier.sync 1, 288;" ::: "memory");   // the epilogue warps may read where it is
+        const uint32_t tmem = tmem_slot;
+        const uint32_t idesc = t5_idesc(128, d.t, a.type == GLMFLASH_BF16);
+        T5Ring at;
+        const uint64_t desc0 = t5_desc(smem_u32(ring));
+        const uint32_t next = d.t * 128 >> 4;
+        const int chain = (mine + d.chains - 1) / d.chains;
+        int in_chain = 0;
+        uint32_t acc = tmem;
+        for (int it = 0; it < mine && ok; ++it) {
+            ok = __all_sync(0xffffffffu, t5_wait<0>(full + at.slot, at.parity, abort_flag, status, GF_STATUS_MMA_TIMEOUT));
+            if (!ok) break;
+            t5_fence_after();
+            const uint64_t da = desc0 + at.slot * (bytes >> 4), db = da + (MATS * DW_A >> 4);
+            if (in_chain == chain) {                         // the next sum
+                in_chain = 0;
+                acc += d.t;
+            }
+            // (A stage is always multiplied whole, zeros behind K and all: a branch around each product made each take 200 clocks.)
+            if (t5_elect()) {
+#pragma unroll
+                for (int m = 0; m < MATS; ++m)
+#pragma unroll
+                    for (int k = 0; k < DW_K / 16; ++k)
+                        t5_mma<1>(acc + m * d.chains * d.t, da + m * (DW_A >> 4) + 2 * (k & 3) + (k >> 2) * (128 * 128 >> 4), db + 2 * (k & 3) + (k >> 2) * next, idesc,
+                                  k > 0 ? 1u : in_chain > 0);
+                t5_commit<1>(done + at.slot);
+                if (it == mine - 1) t5_commit<1>(&acc_full);
+            }
+            __syncwarp();
+            ++in_chain;
+            at.next(d.depth);
+        }
+    } else if (warp >= 4) {
+        pdl_wait();
+        asm volatile("barrier.sync 1, 288;" ::: "memory");
+    }
+    __syncwarp();
+    // The four rows `four` are finished by CTA four % cn, as its slot four / cn (counted along: a division takes 40 instructions).
+    const int live = min(d.t, a.rows - r0), fours = (live + 3) >> 2, q = warp & 3, half = (warp - 4) >> 2, col = (tid - 128) & 127, n = n0 + col;
+    const int groups = (live + 31) >> 5, from = half ? (groups + 1) >> 1 : 0, to = half ? groups : (groups + 1) >> 1;
+    uint32_t slot = 8 * from / cn, owner = 8 * from % cn;
+    float b[2] = {0.f, 0.f};
+    if (warp >= 4) {
+        dense_biases<MATS>(a, n, b);
+        ok = __all_sync(0xffffffffu, t5_wait<100>(&acc_full, 0, abort_flag, status, GF_STATUS_MMA_TIMEOUT));
+        t5_fence_after();
+    }
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (d.alias) cluster_sync();                             // every CTA has multiplied: the ring is free
+    if (warp >= 4 && ok) {
+        const int chain = (mine + d.chains - 1) / d.chains, used = (mine + chain - 1) / chain;      // sums that stages fell to
+        const uint32_t lanes = tmem_slot + ((uint32_t)(q * 32) << 16);
+#pragma unroll 1
+        for (int j = from; j < to; ++j) {
+            float v[MATS][32];
+#pragma unroll
+            for (int m = 0; m < MATS; ++m) {
+                const uint32_t at = lanes + m * d.chains * d.t + 32 * j;
+                t5_ld32(at, v[m]);
+#pragma unroll 1
+                for (int c = 1; c < used; ++c) {
+                    float w[32];
+                    t5_ld32(at + c * d.t, w);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[m][i] += w[i];
+                }
+            }
+            const uint32_t here = smem_u32(parts + rank * d.slots * MATS * 128 + col);
+#pragma unroll
+            for (int g = 0; g < 8; ++g) {
+                if (8 * j + g < fours) {
+                    uint32_t peer;
+                    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(here + slot * (MATS * 2048)), "r"(owner));
+#pragma unroll
+                    for (int m = 0; m < MATS; ++m)
+                        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(peer + m * 2048), "f"(v[m][4 * g]), "f"(v[m][4 * g + 1]),
+                                     "f"(v[m][4 * g + 2]), "f"(v[m][4 * g + 3]) : "memory");
+                }
+                if (++owner == cn) { owner = 0; ++slot; }
+            }
+        }
+    }
+    t5_fence_before();
+    const bool sound = !*abort_flag;
+    __syncwarp();
+    cluster_sync();                                          // the parts of all CTAs have come in
+    t5_fence_after();
+    if (warp == 1) t5_dealloc<1>(tmem_slot, d.cols);
+    if (warp < 4 || !sound || n >= a.N) return;
+#pragma unroll 1
+    for (int s = half; s * (int)cn + rank < fours; s += 2) {
+        float v[MATS][4];
+        const float4 *p = parts + s * MATS * 128 + col;
+#pragma unroll
+        for (int m = 0; m < MATS; ++m) *reinterpret_cast<float4 *>(v[m]) = p[m * 128];
+#pragma unroll 1
+        for (int c = 1; c < (int)cn; ++c) {
+            p += d.slots * MATS * 128;
+#pragma unroll
+            for (int m = 0; m < MATS; ++m) {
+                const float4 w = p[m * 128];
+                v[m][0] += w.x; v[m][1] += w.y; v[m][2] += w.z; v[m][3] += w.w;
+            }
+        }
+        const int r = (s * (int)cn + rank) * 4;
+        dense_finish<MATS>(a, r0 + r, n, min(4, live - r), v[0], v[MATS - 1], b);
+    }
 }
 
-int dense_wide(cudaStream_t s, const DenseArgs &a, bool pdl) {
-    static int sms[64] = {};                               // (threads that come here together set the same)
+// [rows][stride] of 16-bit elements: copies of `box` rows x 64 elements, or x 128 as two blocks of 64 (copies == 1)
+static int dense_map(CUtensorMap *map, const void *base, bool bf, int64_t rows, int K, int64_t stride, int box, int copies, const char *what) {
+    const auto type = bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const uint32_t boxes[3] = {64, (uint32_t)box, 2};
+    const uint64_t blocks[3] = {64, (uint64_t)rows, (uint64_t)K / 64}, dims[2] = {(uint64_t)K, (uint64_t)rows}, strides[2] = {(uint64_t)stride * 2, 128};
+    return encode_map(map, type, copies == 1 ? 3 : 2, const_cast<void *>(base), copies == 1 ? blocks : dims, strides, boxes, what);
+}
+
+// What a device holds: SMs, and clusters of each size (one CTA an SM; they do not span its clusters of SMs).
+struct DenseDevice { int sms, clusters[9]; };
+static int dense_device(const DenseDevice **out) {
+    static DenseDevice known[64] = {};                       // (threads that come here together set the same)
     int dev = 0;
     GF_CUDA(cudaGetDevice(&dev));
     GF_REQUIRE(dev >= 0 && dev < 64, "device ordinal out of range");
-    if (!sms[dev]) {
-        int n = 0;
-        GF_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
-        GF_CUDA(cudaFuncSetAttribute(dense_wide_kernel<1, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)DW_SMEM));
-        GF_CUDA(cudaFuncSetAttribute(dense_wide_kernel<1, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)DW_SMEM));
-        GF_CUDA(cudaFuncSetAttribute(dense_wide_kernel<2, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)DW_SMEM));
-        GF_CUDA(cudaFuncSetAttribute(dense_wide_kernel<2, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)DW_SMEM));
-        sms[dev] = n;
+    if (!known[dev].sms) {
+        for (auto k : {dense_wide_kernel<1, false>, dense_wide_kernel<1, true>, dense_wide_kernel<2, false>, dense_wide_kernel<2, true>})
+            GF_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)DW_SMEM));
+        for (auto k : {dense_thin_kernel<1>, dense_thin_kernel<2>}) GF_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, DT_SMEM));
+        DenseDevice d = {};
+        GF_CUDA(cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev));
+        for (int cn = 1; cn <= 8; ++cn) {
+            cudaLaunchConfig_t cfg = {};
+            cudaLaunchAttribute at[1];
+            at[0].id = cudaLaunchAttributeClusterDimension;
+            at[0].val.clusterDim.x = (unsigned)cn;
+            at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+            cfg.gridDim = dim3((unsigned)(cn * d.sms));
+            cfg.blockDim = dim3(DT_THREADS);
+            cfg.dynamicSmemBytes = DT_SMEM;
+            cfg.attrs = at;
+            cfg.numAttrs = 1;
+            GF_CUDA(cudaOccupancyMaxActiveClusters(&d.clusters[cn], dense_thin_kernel<1>, &cfg));
+        }
+        for (int cn = 1; cn <= 8; ++cn) known[dev].clusters[cn] = d.clusters[cn];
+        known[dev].sms = d.sms;
     }
-    const int pairs = sms[dev] / 2, mats = a.w[1] ? 2 : 1;
-    const bool chain = a.out_type == GLMFLASH_F32 && a.K > DW_CHAIN * 64, bf = a.type == GLMFLASH_BF16;
-    DenseTiles d;
+    *out = &known[dev];
+    return 0;
+}
+
+static int dense_maps(DenseMaps *maps, const DenseArgs &a, int x_box, int copies) {
+    const bool bf = a.type == GLMFLASH_BF16;
+    if (dense_map(&maps->w[0], a.w[0], bf, a.N, a.K, a.ws[0], 128, copies, "weights") || dense_map(&maps->x, a.x, bf, a.rows, a.K, a.xs, x_box, copies, "rows")) return -1;
+    if (a.w[1]) return dense_map(&maps->w[1], a.w[1], bf, a.N, a.K, a.ws[1], 128, copies, "weights");
+    maps->w[1] = maps->w[0];
+    return 0;
+}
+
+int dense_gemm(cudaStream_t s, const DenseArgs &a, bool pdl) {
+    const DenseDevice *device;
+    if (dense_device(&device)) return -1;
+    const int pairs = device->sms / 2, mats = a.w[1] ? 2 : 1, stages = (a.K + DW_K - 1) / DW_K, copies = a.K % 64 ? 2 : 1;
+    const bool chain = a.out_type == GLMFLASH_F32 && stages > DW_CHAIN;
+    // Wide: rows of a tile, what makes the rounds of tiles over the pairs shortest.  A stage of a round takes 234 ns with 32 rows, 244 with 64, 280
+    // with 128, 312 with 192 (the copies bound it: 42 to 50 bytes a clock and SM) and 386 with 256 (1.61 PFLOP/s: the power limit).
+    DenseTiles d = {};
     d.across = (a.N + 255) / 256;
-    // Rows of a tile: what makes the rounds of tiles over the pairs shortest.  A stage of a round takes 234 ns with 32 rows, 244 with 64, 280 with
-    // 128, 312 with 192 (the copies bound it: 42 to 50 bytes a clock and SM) and 386 with 256 (1.61 PFLOP/s: the power limit).
-    int64_t best = INT64_MAX;
-    for (int bn = 32; bn <= DW_ROWS; bn += 32) {        // (N of a pair's product goes in 32)
-        const int64_t tiles = (int64_t)((a.rows + bn - 1) / bn) * d.across, cost = (tiles + pairs - 1) / pairs * std::max(440 + bn, 260 + 2 * bn);
-        if (cost <= best && tiles <= INT32_MAX / 2) { best = cost; d.bn = bn; d.tiles = (int)tiles; }
+    d.stages = stages;
+    d.pass = chain ? DW_CHAIN : stages;
+    double wide = 1e30;
+    for (int bn = 32; bn <= DW_ROWS; bn += 32) {             // (N of a pair's product goes in 32)
+        const int64_t tiles = (int64_t)((a.rows + bn - 1) / bn) * d.across;
+        const double ns = 5500. + (double)((tiles + pairs - 1) / pairs) * stages * mats * std::max({200. + 75. * (copies - 1), (DW_A + bn * 128) / 110., 2.7 * bn}) + bn * 12.;
+        if (ns <= wide && tiles <= INT32_MAX / 2) { wide = ns; d.bn = bn; d.tiles = (int)tiles; }
     }
-    GF_REQUIRE(best != INT64_MAX, "rows * outputs is too large");
-    d.stages = (a.K + 63) / 64;
-    d.pass = chain ? DW_CHAIN : d.stages;
-    const int64_t passes = (int64_t)d.tiles / pairs * mats * d.stages;
-    GF_REQUIRE(passes < INT32_MAX, "product is too large");
+    GF_REQUIRE(wide < 1e30 && (int64_t)(d.tiles / pairs + 1) * mats * stages < INT32_MAX, "the product is too large");
+    // Thin: rows of a tile and CTAs that cut K.
+    DenseThin h = {};
+    int cluster = 0;
+    double thin = 1e30;
+    const int across = (a.N + 127) / 128;
+    for (int tiles = 1; tiles <= 64; ++tiles) {
+        const int t = ((a.rows + tiles - 1) / tiles + 15) / 16 * 16, row_tiles = (a.rows + t - 1) / t;
+        if (t > 256 || row_tiles < tiles) continue;
+        for (int cn = 1; cn <= 8 && cn <= stages; ++cn) {
+            if ((int64_t)across * row_tiles > device->clusters[cn]) continue;
+            const int most = (stages + cn - 1) / cn, chains = chain ? (most + DW_CHAIN - 1) / DW_CHAIN : 1, bytes = mats * DW_A + t * DW_K * 2;
+            const int slots = (t / 4 + cn - 1) / cn, parts = cn * slots * mats * 2048, need = mats * chains * t + (t % 32 ? 16 : 0);
+            if (need > 512 || parts > DT_SMEM - 1024) continue;
+            const int room = DT_SMEM - 1024 - parts, apart = std::min(room / bytes, most);
+            const bool alias = apart < std::min(3, most);
+            const int depth = std::min({alias ? (DT_SMEM - 1024) / bytes : apart, most, DT_DEPTH});
+            if (depth < std::min(2, most)) continue;
+            const double ns = 4000. + most * std::max(170. + 37. * (mats + 1) * copies, bytes / 115.) + (alias ? 400. : 0.) + t * mats * 8. + slots * mats * (20. + 15. * cn);
+            if (ns < thin) {
+                thin = ns;
+                cluster = cn;
+                h = {t, row_tiles, stages, chains, depth, copies, slots, alias, need <= 32 ? 32 : need <= 64 ? 64 : need <= 128 ? 128 : need <= 256 ? 256 : 512};
+            }
+        }
+    }
     DenseMaps maps;
-    if (dense_map(&maps.w[0], a.w[0], bf, a.N, a.K, a.ws[0], 128, "weights")) return -1;
-    if (mats == 2 && dense_map(&maps.w[1], a.w[1], bf, a.N, a.K, a.ws[1], 128, "weights")) return -1;
-    if (mats == 1) maps.w[1] = maps.w[0];
-    if (dense_map(&maps.x, a.x, bf, a.rows, a.K, a.xs, d.bn / 2, "rows")) return -1;
-    const dim3 grid((unsigned)(2 * std::min(d.tiles, pairs))), block(DW_THREADS);
+    if (thin < wide) {
+        if (dense_maps(&maps, a, h.t, copies)) return -1;
+        const int bytes = mats * DW_A + h.t * DW_K * 2, parts = cluster * h.slots * mats * 2048;
+        const size_t smem = 1024 + (h.alias ? std::max(h.depth * bytes, parts) : h.depth * bytes + parts);
+        return launch_kc(mats == 2 ? dense_thin_kernel<2> : dense_thin_kernel<1>, dim3((unsigned)(across * h.row_tiles * cluster)), dim3(DT_THREADS),
+                         dim3((unsigned)cluster), smem, s, pdl, maps, a, h);
+    }
+    d.copies = copies;
+    d.depth = std::min(DW_RING / (DW_A + d.bn * 128), DW_DEPTH);
+    if (dense_maps(&maps, a, d.bn / 2, copies)) return -1;
     auto kernel = mats == 2 ? (chain ? dense_wide_kernel<2, true> : dense_wide_kernel<2, false>) : (chain ? dense_wide_kernel<1, true> : dense_wide_kernel<1, false>);
-    return launch_k(kernel, grid, block, DW_SMEM, s, pdl, maps, a, d);
+    return launch_k(kernel, dim3((unsigned)(2 * std::min(d.tiles, pairs))), dim3(DW_THREADS), DW_SMEM, s, pdl, maps, a, d);
 }
 
 }  // namespace gf

@@ -84,14 +84,23 @@ __device__ __forceinline__ uint32_t t5_of_cta(const void *p, uint32_t cta) {
     return r;
 }
 __device__ __forceinline__ void t5_arrive_cluster(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
-// tensor copy of one CTA of a pair; its bytes count on a barrier of either CTA, named by its address in the cluster
-__device__ __forceinline__ void t5_load_pair(void *dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
-    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-                 ::"r"(smem_u32(dst)), "l"((uint64_t)map), "r"(x), "r"(y), "r"(bar) : "memory");
+// Tensor copies of 64-element blocks k, k + 1, .. of the rows from y on: a box of several blocks (three dimensions), or of one (two).
+// Of a pair: its bytes count on a barrier of either CTA, named by its address in the cluster.
+__device__ __forceinline__ void t5_load_pair(void *dst, const CUtensorMap *map, bool blocks, int k, int y, uint32_t bar) {
+    if (blocks)
+        asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                     ::"r"(smem_u32(dst)), "l"((uint64_t)map), "r"(0), "r"(y), "r"(k), "r"(bar) : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                     ::"r"(smem_u32(dst)), "l"((uint64_t)map), "r"(64 * k), "r"(y), "r"(bar) : "memory");
 }
-__device__ __forceinline__ void t5_load(void *dst, const CUtensorMap *map, int x, int y, uint64_t *bar) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-                 ::"r"(smem_u32(dst)), "l"((uint64_t)map), "r"(x), "r"(y), "r"(smem_u32(bar)) : "memory");
+__device__ __forceinline__ void t5_load(void *dst, const CUtensorMap *map, bool blocks, int k, int y, uint64_t *bar) {
+    if (blocks)
+        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                     ::"r"(smem_u32(dst)), "l"((uint64_t)map), "r"(0), "r"(y), "r"(k), "r"(smem_u32(bar)) : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                     ::"r"(smem_u32(dst)), "l"((uint64_t)map), "r"(64 * k), "r"(y), "r"(smem_u32(bar)) : "memory");
 }
 
 // Wait for a phase.  Gives up when the CTA's abort flag is up, when another CTA has set the status word, or after a number of polls (seconds);
