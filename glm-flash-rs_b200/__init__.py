@@ -578,28 +578,46 @@ def _named(table, name, what):
     return table[name]
 
 
+_calls = None
+
+
+def _hot():
+    """(current device, current raw stream, topk_by, route_by, linear): looked up once, since a small call's lookups cost as much as its kernel."""
+    global _calls
+    if _calls is None:
+        c, L = _torch()._C, lib()
+        _calls = c._cuda_getDevice, c._cuda_getCurrentRawStream, L.glmflash_topk_by, L.glmflash_route_by, L.glmflash_linear
+    return _calls
+
+
 @functools.lru_cache(maxsize=256)
 def _rule(scores, groups, keep_groups, group_score, renorm, scale):
     return _RULE.pack(_named(SCORES, scores, "scores"), groups, groups if keep_groups is None else keep_groups,
                       _named(GROUP_SCORES, group_score, "group_score"), int(bool(renorm)), scale, 0, 0)
 
 
-def _table_args(logits, picks, weights, bias):
-    """Checks of a selection's tensors; (rows, experts, device index)."""
+def _table_refusal(logits, picks, weights, bias, dev):
+    """What is wrong with a selection's tensors."""
     torch = _torch()
     _require(logits.dim() == 2 and picks.dim() == 2 and weights.dim() == 2, "logits, picks and weights must have two dimensions")
     rows, E = logits.shape
-    dev = logits.get_device()
-    _require(dev == torch._C._cuda_getDevice(), "tensors must be on the current CUDA device")
+    _require(logits.get_device() == dev, "tensors must be on the current CUDA device")
     _require(logits.dtype is torch.float32 and picks.dtype is torch.int32 and weights.dtype is torch.float32,
              "logits and weights must be float32, picks int32")
     _require(picks.get_device() == dev and weights.get_device() == dev, "tensors must be on one device")
     _require(picks.shape == weights.shape and picks.shape[0] == rows, "picks and weights must be [rows][topk + 1]")
     _require(picks.is_contiguous() and weights.is_contiguous(), "picks and weights must be contiguous")
-    if bias is not None:
-        _require(bias.dtype is torch.float32 and bias.dim() == 1 and bias.shape[0] == E and bias.get_device() == dev and
-                 (bias.stride(0) == 1 or E == 1), "bias must be float32 [experts], contiguous, on the same device")
-    return rows, E, dev
+    _require(bias is None or (bias.dtype is torch.float32 and bias.shape == (E,) and bias.get_device() == dev and bias.is_contiguous()),
+             "bias must be float32 [experts], contiguous, on the same device")
+    raise GlmFlashError("logits must have neighbouring experts side by side")
+
+
+def _table_fits(logits, picks, weights, bias, dev):
+    f32, shape, table = _cuda_torch.float32, logits.shape, picks.shape
+    return (logits.dtype is f32 and weights.dtype is f32 and picks.dtype is _cuda_torch.int32 and len(shape) == 2 and len(table) == 2 and
+            weights.shape == table and table[0] == shape[0] and logits.get_device() == dev and picks.get_device() == dev and
+            weights.get_device() == dev and picks.is_contiguous() and weights.is_contiguous() and
+            (bias is None or (bias.dtype is f32 and bias.shape == shape[1:] and bias.get_device() == dev and bias.is_contiguous())))
 
 
 def topk_by(logits, picks, weights, bias=None, scores="sigmoid", groups=1, keep_groups=None, group_score="max", renorm=True, scale=1.0,
@@ -607,30 +625,43 @@ def topk_by(logits, picks, weights, bias=None, scores="sigmoid", groups=1, keep_
     """Routing table of logits fp32 [rows][E] by a rule (glmflash_topk_by): `scores` "sigmoid" or "softmax", `bias` fp32 [E] added to them
     for the choice alone, `groups` of neighbouring experts of which the `keep_groups` best by `group_score` ("max" or "top2") stay, weights
     renormalised or not and times `scale`.  Writes picks int32 / weights fp32 [rows][k + 1] (shared expert last) and returns them."""
-    rows, E, _ = _table_args(logits, picks, weights, bias)
-    _require(logits.stride(1) == 1 or E == 1, "logits must have neighbouring experts side by side")
-    _check(lib().glmflash_topk_by(_stream_ptr(stream), logits.data_ptr(), logits.stride(0) if rows > 1 else E,
-                                  None if bias is None else bias.data_ptr(), rows, E, picks.shape[1] - 1,
-                                  _rule(scores, groups, keep_groups, group_score, renorm, scale), _RULE.size, picks.data_ptr(),
-                                  weights.data_ptr(), pdl))
+    get_device, get_stream, call, _, _ = _calls or _hot()
+    dev = get_device()
+    if not _table_fits(logits, picks, weights, bias, dev):
+        _table_refusal(logits, picks, weights, bias, dev)
+    rows, E = logits.shape
+    step, side = logits.stride()
+    if side != 1 and E > 1:
+        _table_refusal(logits, picks, weights, bias, dev)
+    if call(get_stream(dev) if stream is None else stream.cuda_stream, logits.data_ptr(), step if rows > 1 else E, None if bias is None else bias.data_ptr(),
+            rows, E, picks.shape[1] - 1, _rule(scores, groups, keep_groups, group_score, renorm, scale), _RULE.size, picks.data_ptr(), weights.data_ptr(), pdl):
+        _check(-1)
     return picks, weights
 
 
 def route_by(x, wr, logits, picks, weights, bias=None, scores="sigmoid", groups=1, keep_groups=None, group_score="max", renorm=True,
              scale=1.0, stream=None, pdl=1):
     """router_logits + topk_by: x bf16 [rows][hidden], wr bf16 [E][hidden]; fills logits, picks and weights."""
-    torch = _torch()
-    rows, E, dev = _table_args(logits, picks, weights, bias)
-    _require(logits.is_contiguous(), "logits must be contiguous")
-    _require(x.dim() == 2 and wr.dim() == 2 and x.shape[0] == rows and wr.shape[0] == E and x.shape[1] == wr.shape[1],
-             "x must be [rows][hidden] and the router matrix [experts][hidden]")
-    _require(x.dtype is torch.bfloat16 and wr.dtype is torch.bfloat16, "x and the router matrix must be bfloat16")
-    _require(x.get_device() == dev and wr.get_device() == dev, "tensors must be on one device")
-    _require(x.stride(1) == 1 and wr.is_contiguous(), "rows of x and the router matrix must be contiguous")
-    _check(lib().glmflash_route_by(_stream_ptr(stream), x.data_ptr(), x.stride(0) if rows > 1 else x.shape[1], wr.data_ptr(),
-                                   None if bias is None else bias.data_ptr(), rows, wr.shape[1], E, picks.shape[1] - 1,
-                                   _rule(scores, groups, keep_groups, group_score, renorm, scale), _RULE.size, logits.data_ptr(),
-                                   picks.data_ptr(), weights.data_ptr(), pdl))
+    get_device, get_stream, _, call, _ = _calls or _hot()
+    dev, bf16 = get_device(), _cuda_torch.bfloat16
+    if not (_table_fits(logits, picks, weights, bias, dev) and logits.is_contiguous()):
+        _require(logits.is_contiguous(), "logits must be contiguous")
+        _table_refusal(logits, picks, weights, bias, dev)
+    (rows, E), xshape, wshape = logits.shape, x.shape, wr.shape
+    if not (len(xshape) == 2 and xshape[0] == rows and wshape == (E, xshape[1])):
+        raise GlmFlashError("x must be [rows][hidden] and the router matrix [experts][hidden]")
+    if x.dtype is not bf16 or wr.dtype is not bf16:
+        raise GlmFlashError("x and the router matrix must be bfloat16")
+    if x.get_device() != dev or wr.get_device() != dev:
+        raise GlmFlashError("tensors must be on one device")
+    step, side = x.stride()
+    H = xshape[1]
+    if not (side == 1 or H == 1) or not wr.is_contiguous():
+        raise GlmFlashError("rows of x and the router matrix must be contiguous")
+    if call(get_stream(dev) if stream is None else stream.cuda_stream, x.data_ptr(), step if rows > 1 else H, wr.data_ptr(),
+            None if bias is None else bias.data_ptr(), rows, H, E, picks.shape[1] - 1, _rule(scores, groups, keep_groups, group_score, renorm, scale),
+            _RULE.size, logits.data_ptr(), picks.data_ptr(), weights.data_ptr(), pdl):
+        _check(-1)
     return picks, weights
 
 
@@ -638,60 +669,90 @@ _TYPE_CODES = {}
 
 
 def _type_codes():
-    if not _TYPE_CODES:
-        torch = _torch()
-        _TYPE_CODES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+    torch = _torch()
+    _TYPE_CODES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
     return _TYPE_CODES
 
 
-def _dense(x, w, w_up, out, bias, bias_up, act, residual, out_dtype, limit, stream, pdl):
+def _vector(b, N, dt, dev):
+    """A bias's type code and address."""
+    code = _TYPE_CODES.get(b.dtype, -1)
+    _require(b.shape == (N,) and b.get_device() == dev and b.is_contiguous(), "a bias must be [outer], contiguous, on x's device")
+    _require(code == 0 or b.dtype is dt, "a bias must be float32 or of x's type")
+    return code, b.data_ptr()
+
+
+def _matrix(t, rows, cols, dt, dev, what):
+    """A residual's or output's type code, address and stride."""
+    code = _TYPE_CODES.get(t.dtype, -1)
+    if t.shape != (rows, cols) or t.get_device() != dev:
+        raise GlmFlashError(what + " must be [rows][outer] on x's device")
+    if code and t.dtype is not dt:
+        raise GlmFlashError(what + " must be float32 or of x's type")
+    step, side = t.stride()
+    if side != 1 and cols > 1:
+        raise GlmFlashError(what + " must have the elements of a row side by side")
+    return code, t.data_ptr(), step if rows > 1 else cols
+
+
+def _operands(x, w, w_up, dev):
+    """What is wrong with x and the weights."""
     torch = _torch()
-    codes, dt, dev = _type_codes(), x.dtype, x.get_device()
-    _require(dev == torch._C._cuda_getDevice(), "tensors must be on the current CUDA device")
+    _require(x.get_device() == dev, "tensors must be on the current CUDA device")
     _require(x.dim() == 2 and w.dim() == 2 and x.shape[1] == w.shape[1], "x must be [rows][inner] and the weights [outer][inner]")
-    rows, K = x.shape
-    N = w.shape[0]
-    _require(rows > 0 and K > 0 and N > 0, "rows, inner and outer must be positive")
-    _require(dt is torch.float16 or dt is torch.bfloat16, "x and the weights must be float16 or bfloat16")
-    ws = us = up = 0
-    for m in (w,) if w_up is None else (w, w_up):
-        _require(m.shape == w.shape and m.dtype is dt and m.get_device() == dev, "the weights must have x's type and device and one shape")
-        _require(m.stride(1) == 1 or K == 1, "the weights must have neighbouring inputs side by side")
-    ws = w.stride(0) if N > 1 else -(-K // 8) * 8          # (the stride of a single row is never used)
+    _require(x.shape[0] > 0 and x.shape[1] > 0 and w.shape[0] > 0, "rows, inner and outer must be positive")
+    _require(x.dtype is torch.float16 or x.dtype is torch.bfloat16, "x and the weights must be float16 or bfloat16")
+    for m in (w, w if w_up is None else w_up):
+        _require(m.shape == w.shape and m.dtype is x.dtype and m.get_device() == dev, "the weights must have x's type and device and one shape")
+    raise GlmFlashError("x and the weights must have the elements of a row side by side")
+
+
+def _dense(x, w, w_up, out, bias, bias_up, act, residual, out_dtype, limit, stream, pdl):
+    get_device, get_stream, _, _, call = _calls or _hot()
+    codes = _TYPE_CODES or _type_codes()
+    dt, dev, xshape, wshape = x.dtype, get_device(), x.shape, w.shape
+    code = codes.get(dt, 0)
+    if not (code and len(xshape) == 2 and len(wshape) == 2 and xshape[1] == wshape[1] and w.dtype is dt and x.get_device() == dev and w.get_device() == dev):
+        _operands(x, w, w_up, dev)
+    rows, K = xshape
+    N = wshape[0]
+    (xs, side), (ws, w_side) = x.stride(), w.stride()
+    if not (rows and K and N and (K == 1 or (side == 1 and w_side == 1))):
+        _operands(x, w, w_up, dev)
+    whole = -(-K // 8) * 8                                 # (the stride of a single row is never used)
+    if rows == 1:
+        xs = whole
+    if N == 1:
+        ws = whole
+    us = up = bt = bp = bu = rt = rp = rs = 0
     if w_up is not None:
-        us, up = w_up.stride(0) if N > 1 else ws, w_up.data_ptr()
-    _require(x.stride(1) == 1 or K == 1, "x must have the elements of a row side by side")
-    xs = x.stride(0) if rows > 1 else -(-K // 8) * 8
+        us, side = w_up.stride() if w_up.dim() == 2 else (0, 0)
+        if w_up.shape != wshape or w_up.dtype is not dt or w_up.get_device() != dev or (side != 1 and K > 1):
+            _operands(x, w, w_up, dev)
+        up = w_up.data_ptr()
+        if N == 1:
+            us = whole
     if out is None:
         if stream is None:
             out = x.new_empty((rows, N), dtype=out_dtype)
         else:                                              # (memory of the stream that writes it)
-            with torch.cuda.stream(stream):
+            with _cuda_torch.cuda.stream(stream):
                 out = x.new_empty((rows, N), dtype=out_dtype)
-    else:
-        _require(out_dtype is None or out_dtype is out.dtype, "out has another type than out_dtype")
-    ot = out.dtype
-    _require(out.shape == (rows, N) and out.get_device() == dev and (out.stride(1) == 1 or N == 1), "out must be [rows][outer] on x's device, a row's elements side by side")
-    _require(ot is dt or ot is torch.float32, "the output must be float32 or of x's type")
-    bt, bp, bu = 0, 0, 0
-    if bias is not None or bias_up is not None:
-        first = bias if bias is not None else bias_up
-        bt = codes.get(first.dtype, -1)
-        for b in (bias, bias_up):
-            _require(b is None or (b.dtype is first.dtype and b.dim() == 1 and b.shape[0] == N and b.get_device() == dev and (b.stride(0) == 1 or N == 1)),
-                     "a bias must be [outer], contiguous, on x's device (both of one type)")
-        _require(first.dtype is dt or bt == 0, "a bias must be float32 or of x's type")
-        bp, bu = 0 if bias is None else bias.data_ptr(), 0 if bias_up is None else bias_up.data_ptr()
-    rt = rp = rs = 0
+    elif out_dtype is not None and out_dtype is not out.dtype:
+        raise GlmFlashError("out has another type than out_dtype")
+    ot, op, os_ = _matrix(out, rows, N, dt, dev, "the output")
+    if bias is not None:
+        bt, bp = _vector(bias, N, dt, dev)
+    if bias_up is not None:
+        both, bu = _vector(bias_up, N, dt, dev)
+        _require(bias is None or both == bt, "the biases must be of one type")
+        bt = both
     if residual is not None:
-        rt = codes.get(residual.dtype, -1)
-        _require(residual.shape == (rows, N) and residual.get_device() == dev and (residual.stride(1) == 1 or N == 1),
-                 "the residual must be [rows][outer] on x's device, a row's elements side by side")
-        _require(residual.dtype is dt or rt == 0, "the residual must be float32 or of x's type")
-        rp, rs = residual.data_ptr(), residual.stride(0) if rows > 1 else N
-    args = _LINEAR.pack(x.data_ptr(), w.data_ptr(), up, bp, bu, rp, out.data_ptr(), xs, ws, us, rs, out.stride(0) if rows > 1 else N, rows, K, N, codes[dt],
-                        bt, rt, codes[ot], _named(ACTS, act, "act"), limit, pdl, 0, 0)
-    _check(lib().glmflash_linear(_stream_ptr(stream), args, _LINEAR.size))
+        rt, rp, rs = _matrix(residual, rows, N, dt, dev, "the residual")
+    if call(get_stream(dev) if stream is None else stream.cuda_stream,
+            _LINEAR.pack(x.data_ptr(), w.data_ptr(), up, bp, bu, rp, op, xs, ws, us, rs, os_, rows, K, N, code, bt, rt, ot,
+                         ACTS[act] if act in ACTS else _named(ACTS, act, "act"), limit, pdl, 0, 0), _LINEAR.size):
+        _check(-1)
     return out
 
 

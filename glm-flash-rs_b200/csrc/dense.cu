@@ -23,41 +23,76 @@ __device__ __forceinline__ uint4 dense_piece(const uint16_t *row, int k, int K) 
     return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
-// A CTA has 16 output columns of 8 RT rows; its 8 warps cut K.  The weights are the 16-row operand of mma.m16n8k16, the rows the 8-column
-// one.  The k slots of a fragment may be any as long as both operands agree: a lane loads 16 contiguous bytes of a row (k = 8 t .. 8 t + 7
-// of a 32-k step) and uses them as the fragments of two instructions.
-constexpr int DN_N = 16, DN_WARPS = 8;
+__device__ __forceinline__ uint4 dense_ldg(const void *p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
+// Up to 8 RT rows: bound by the latency of one trip to the weights.  A CTA has 16 output columns, its 16 warps cut K into steps of 32 and ask for
+// several steps each before the first product.  The weights are the 16-row operand of mma.m16n8k16, the rows the 8-column
+// one.  The k slots of a fragment may be any as long as both operands agree: a lane loads 16 contiguous bytes of a row (k = 8 t .. 8 t + 7 of a step) and
+// uses them as the fragments of two instructions.
+constexpr int DN_N = 16, DN_WARPS = 16, DN_AHEAD = 4;
 template <bool BF, int MATS, int RT>
-__global__ void __launch_bounds__(DN_WARPS * 32) dense_kernel(const DenseArgs a, int row_tiles) {
+__global__ void __launch_bounds__(DN_WARPS * 32, MATS * RT == 1 ? 2 : 1) dense_kernel(const DenseArgs a) {
     __shared__ float part[DN_WARPS][MATS][8 * RT][DN_N + 1];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int n0 = blockIdx.x * DN_N, whole = a.K >> 5;
+    const uint16_t *w[MATS][2];
+#pragma unroll
+    for (int m = 0; m < MATS; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) w[m][h] = static_cast<const uint16_t *>(a.w[m]) + min(n0 + 8 * h + g, a.N - 1) * a.ws[m] + 8 * t;   // (columns behind the last: the last's)
+#pragma unroll
+    for (int m = 0; m < MATS; ++m)                           // (a hint: the lines are on their way to L2 while the kernel in front ends)
+#pragma unroll
+        for (int i = 0; i < DN_AHEAD; ++i)
+            if (warp + DN_WARPS * i < whole) {
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(w[m][0] + (warp + DN_WARPS * i) * 32));
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(w[m][1] + (warp + DN_WARPS * i) * 32));
+            }
     pdl_wait();
     pdl_launch_dependents();
-    const int n0 = (int)(blockIdx.x / row_tiles) * DN_N, r0 = (int)(blockIdx.x % row_tiles) * 8 * RT;
+    const uint16_t *x = static_cast<const uint16_t *>(a.x) + g * a.xs + 8 * t;
     float acc[MATS][RT][4] = {};
     const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-    for (int s = warp; s * 32 < a.K; s += DN_WARPS) {
-        const int k = s * 32 + 8 * t;
-        uint4 xv[RT];
+    auto multiply = [&](const uint4 (&wv)[MATS][2], const uint4 (&xv)[RT]) {
 #pragma unroll
-        for (int i = 0; i < RT; ++i) {
-            const int r = r0 + 8 * i + g;
-            xv[i] = r < a.rows && k < a.K ? dense_piece(static_cast<const uint16_t *>(a.x) + r * a.xs, k, a.K) : zero;
-        }
-#pragma unroll
-        for (int m = 0; m < MATS; ++m) {
-            uint4 wv[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int n = n0 + 8 * h + g;
-                wv[h] = n < a.N && k < a.K ? dense_piece(static_cast<const uint16_t *>(a.w[m]) + n * a.ws[m], k, a.K) : zero;
-            }
+        for (int m = 0; m < MATS; ++m)
 #pragma unroll
             for (int i = 0; i < RT; ++i) {
-                dense_mma<BF>(acc[m][i], wv[0].x, wv[1].x, wv[0].y, wv[1].y, xv[i].x, xv[i].y);
-                dense_mma<BF>(acc[m][i], wv[0].z, wv[1].z, wv[0].w, wv[1].w, xv[i].z, xv[i].w);
+                dense_mma<BF>(acc[m][i], wv[m][0].x, wv[m][1].x, wv[m][0].y, wv[m][1].y, xv[i].x, xv[i].y);
+                dense_mma<BF>(acc[m][i], wv[m][0].z, wv[m][1].z, wv[m][0].w, wv[m][1].w, xv[i].z, xv[i].w);
             }
+    };
+#pragma unroll 1
+    for (int s0 = warp; s0 < whole; s0 += DN_WARPS * DN_AHEAD) {
+        uint4 wv[DN_AHEAD][MATS][2], xv[DN_AHEAD][RT];
+#pragma unroll
+        for (int i = 0; i < DN_AHEAD; ++i) {
+            const int s = s0 + DN_WARPS * i;
+            const bool here = s < whole;
+#pragma unroll
+            for (int m = 0; m < MATS; ++m)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) wv[i][m][h] = here ? dense_ldg(w[m][h] + s * 32) : zero;
+#pragma unroll
+            for (int j = 0; j < RT; ++j) xv[i][j] = here && 8 * j + g < a.rows ? dense_ldg(x + 8 * j * a.xs + s * 32) : zero;
         }
+#pragma unroll
+        for (int i = 0; i < DN_AHEAD; ++i) multiply(wv[i], xv[i]);
+    }
+    if ((a.K & 31) && warp == whole % DN_WARPS) {            // the ragged end of K
+        uint4 wv[MATS][2], xv[RT];
+        const int k = whole * 32 + 8 * t;
+#pragma unroll
+        for (int m = 0; m < MATS; ++m)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) wv[m][h] = k < a.K ? dense_piece(w[m][h] - 8 * t, k, a.K) : zero;
+#pragma unroll
+        for (int j = 0; j < RT; ++j) xv[j] = 8 * j + g < a.rows && k < a.K ? dense_piece(x + 8 * j * a.xs - 8 * t, k, a.K) : zero;
+        multiply(wv, xv);
     }
 #pragma unroll
     for (int m = 0; m < MATS; ++m)
@@ -69,28 +104,34 @@ __global__ void __launch_bounds__(DN_WARPS * 32) dense_kernel(const DenseArgs a,
             part[warp][m][8 * i + 2 * t + 1][g + 8] = acc[m][i][3];
         }
     __syncthreads();
-    if (tid >= 8 * RT * DN_N) return;
     const int r = tid / DN_N, n = tid % DN_N;
-    if (r0 + r >= a.rows || n0 + n >= a.N) return;
+    if (tid >= 8 * RT * DN_N || r >= a.rows || n0 + n >= a.N) return;
     float v[MATS][1], b[2];
     dense_biases<MATS>(a, n0 + n, b);
 #pragma unroll
     for (int m = 0; m < MATS; ++m) {
         v[m][0] = 0.f;
 #pragma unroll
-        for (int w = 0; w < DN_WARPS; ++w) v[m][0] += part[w][m][r][n];
+        for (int k = 0; k < DN_WARPS; ++k) v[m][0] += part[k][m][r][n];
     }
-    dense_finish<MATS>(a, r0 + r, n0 + n, 1, v[0], v[MATS - 1], b);
+    dense_finish<MATS>(a, r, n0 + n, 1, v[0], v[MATS - 1], b);
+}
+
+// Which calls of up to 16 rows it takes: those whose CTAs run at once (two an SM for one matrix and up to 8 rows), with few trips a warp.  us, this
+// kernel | the tensor-memory ones, inner x outer, 1 and 8 rows: 512 x 512 2.1 2.1 | 3.3 3.1; 2048 x 2048 3.1 3.5 | 4.3 4.3; 2048 x 4096 4.3 4.9
+// | 5.2 5.2; 4096 x 4096 6.3 7.8 | 6.6 6.4; 8192 x 1024 6.5 7.0 | 5.6 5.8; 2048 x 8192 8.0 9.1 | 6.6 6.2.  9 and 16 rows: 2048 x 2048 3.4 4.2 |
+// 4.3 4.4; 4096 x 2048 5.6 5.9 | 5.4 5.4; 2048 x 4096 6.2 7.0 | 5.2 5.1.  The gated pair, 1, 8, 9, 16 rows: 2048 x 2048 4.2 4.5 4.9 5.8 | 5.8 5.6
+// 6.0 5.8; 4096 x 2048 5.8 6.2 7.0 7.5 | 7.7 7.5 8.0 7.8; 8192 x 1024 8.1 9.0 10.1 11.0 | 8.5 8.3 8.8 8.6; 2048 x 4096 7.9 8.6 9.2 10.1 | 7.2 6.8 7.2 6.8.
+static bool dense_small(const DenseArgs &a) {
+    if (a.rows > 16 || a.K > 4096 || a.N > 148 * 2 * DN_N) return false;
+    if (a.w[1]) return a.N <= 148 * DN_N;
+    return a.rows <= 8 ? (int64_t)a.K * a.N <= 1 << 23 : a.K <= 2048 && a.N <= 148 * DN_N;
 }
 
 template <bool BF, int MATS>
 static int launch_dense(cudaStream_t s, const DenseArgs &a, bool pdl) {
-    const int rt = a.rows > 8 ? 2 : 1;
-    const int64_t row_tiles = (a.rows + 8 * rt - 1) / (8 * rt), tiles = row_tiles * ((a.N + DN_N - 1) / DN_N);
-    GF_REQUIRE(tiles <= INT32_MAX, "rows * outputs is too large");
-    const dim3 grid((unsigned)tiles), block(DN_WARPS * 32);
-    return rt == 2 ? launch_k(dense_kernel<BF, MATS, 2>, grid, block, 0, s, pdl, a, (int)row_tiles)
-                   : launch_k(dense_kernel<BF, MATS, 1>, grid, block, 0, s, pdl, a, (int)row_tiles);
+    const dim3 grid((unsigned)((a.N + DN_N - 1) / DN_N)), block(DN_WARPS * 32);
+    return a.rows > 8 ? launch_k(dense_kernel<BF, MATS, 2>, grid, block, 0, s, pdl, a) : launch_k(dense_kernel<BF, MATS, 1>, grid, block, 0, s, pdl, a);
 }
 
 }  // namespace gf
@@ -130,7 +171,7 @@ extern "C" int glmflash_linear(void *stream, const glmflash_linear_args *p, size
                    p->out_stride, p->rows, p->inner, p->outer, p->type, p->bias_type, p->residual_type, p->out_type, p->act, p->limit};
     const bool bf = p->type == GLMFLASH_BF16, pdl = p->pdl != 0;
     cudaStream_t s = (cudaStream_t)stream;
-    if (p->rows > 16) return dense_gemm(s, a, pdl);
+    if (!dense_small(a)) return dense_gemm(s, a, pdl);
     if (gated) return bf ? launch_dense<true, 2>(s, a, pdl) : launch_dense<false, 2>(s, a, pdl);
     return bf ? launch_dense<true, 1>(s, a, pdl) : launch_dense<false, 1>(s, a, pdl);
 }

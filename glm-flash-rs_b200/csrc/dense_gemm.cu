@@ -505,7 +505,9 @@ int dense_gemm(cudaStream_t s, const DenseArgs &a, bool pdl) {
     double wide = 1e30;
     for (int bn = 32; bn <= DW_ROWS; bn += 32) {             // (N of a pair's product goes in 32)
         const int64_t tiles = (int64_t)((a.rows + bn - 1) / bn) * d.across;
-        const double ns = 5500. + (double)((tiles + pairs - 1) / pairs) * stages * mats * std::max({200. + 75. * (copies - 1), (DW_A + bn * 128) / 110., 2.7 * bn}) + bn * 12.;
+        const int64_t rounds = (tiles + pairs - 1) / pairs;
+        const double busy = std::min(1., (double)tiles / pairs);
+        const double ns = 5000. + 11. * bn + (double)rounds * stages * mats * std::max({160., 2.05 * bn, busy * (170. + 1.6 * bn)});
         if (ns <= wide && tiles <= INT32_MAX / 2) { wide = ns; d.bn = bn; d.tiles = (int)tiles; }
     }
     GF_REQUIRE(wide < 1e30 && (int64_t)(d.tiles / pairs + 1) * mats * stages < INT32_MAX, "the product is too large");
@@ -526,7 +528,9 @@ int dense_gemm(cudaStream_t s, const DenseArgs &a, bool pdl) {
             const bool alias = apart < std::min(3, most);
             const int depth = std::min({alias ? (DT_SMEM - 1024) / bytes : apart, most, DT_DEPTH});
             if (depth < std::min(2, most)) continue;
-            const double ns = 4000. + most * std::max(170. + 37. * (mats + 1) * copies, bytes / 115.) + (alias ? 400. : 0.) + t * mats * 8. + slots * mats * (20. + 15. * cn);
+            const double mma = mats * 8 * std::max({41., 33. + 0.25 * t, 0.5 * t}) / 1.9 + 130.;
+            const double ns = 2440. + most * (154. + 0.54 * std::max({mma, bytes / 150., bytes * (double)(across * row_tiles * cn) / 9000.})) +
+                              0.0056 * t * mats * 1024. * (cn - 1) / cn + slots * mats * (88. + 74. * cn);
             if (ns < thin) {
                 thin = ns;
                 cluster = cn;
