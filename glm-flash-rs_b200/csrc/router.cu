@@ -244,20 +244,23 @@ __global__ void __launch_bounds__(256) route_kernel(const __nv_bfloat16 *__restr
 }
 
 constexpr int SEL_WARPS = 4;
-__global__ void __launch_bounds__(SEL_WARPS * 32) select_kernel(const float *logits, int64_t stride, const float *bias, int rows, int E, int topk,
-                                                                SelRule rule, int *picks, float *weights) {
+__global__ void __launch_bounds__(SEL_WARPS * 32, 8) select_kernel(const float *logits, int64_t stride, const float *bias, int rows, int E, int topk, SelRule rule,
+                                                                   int *picks, float *weights) {
     extern __shared__ double sel_values[];
+    __shared__ int2 spot[SEL_WARPS][32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.x * SEL_WARPS + warp;
     pdl_wait();
     pdl_launch_dependents();
     if (r >= rows) return;
-    select_row(logits + r * stride, bias, E, topk, rule, sel_values + (size_t)warp * E, picks + (size_t)r * (topk + 1), weights + (size_t)r * (topk + 1), lane);
+    select_row(logits + r * stride, bias, E, topk, rule, sel_values + warp * (bias ? (E + 31) / 32 * 32 : (E + 31) / 32 * 16), spot[warp],
+               picks + (size_t)r * (topk + 1), weights + (size_t)r * (topk + 1), lane);
 }
 
 static int launch_select(cudaStream_t s, const float *logits, int64_t stride, const float *bias, int rows, int E, int topk, const SelRule &rule, int *picks,
                          float *weights, bool pdl) {
-    return launch_k(select_kernel, dim3((unsigned)((rows + SEL_WARPS - 1) / SEL_WARPS)), dim3(SEL_WARPS * 32), (size_t)SEL_WARPS * E * sizeof(double), s, pdl,
-                    logits, stride, bias, rows, E, topk, rule, picks, weights);
+    const dim3 grid((unsigned)((rows + SEL_WARPS - 1) / SEL_WARPS)), block(SEL_WARPS * 32);
+    const size_t smem = (size_t)SEL_WARPS * ((E + 31) / 32 * 32) * (bias ? sizeof(double) : sizeof(float));
+    return launch_k(select_kernel, grid, block, smem, s, pdl, logits, stride, bias, rows, E, topk, rule, picks, weights);
 }
 
 static int launch_route(cudaStream_t s, const uint16_t *x, int x_stride, const uint16_t *wr, int rows, int H, int E, int topk, float *logits,

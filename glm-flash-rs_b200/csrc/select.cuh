@@ -3,13 +3,15 @@
 //
 //   l = the logit, -inf where it is NaN;  s = 1 / (1 + exp(-l)) or exp(l - max) / sum exp(l - max)
 //   c = s + bias (-inf where the bias is NaN);  without a bias c = l, whose order is that of the scores
-//   value of a group = its largest c, or the sum of its two largest c (without a bias: s); the largest groups stay, ties to the lower one
+//   value of a group = its largest c, or the sum of its two largest c (without a bias: s; +inf where one is); the largest groups stay, ties to
+//   the lower one
 //   choice = the topk largest c of the groups that stay, descending, ties to the lower id
 //   weight = s * scale, or s / (sum of the chosen s) * scale, 0 where that sum is 0
 // A softmax row whose largest logit is +inf shares 1 among its infinities (the limit); one without a logit above -inf has scores of 0.
 // So every row gets topk different ids of the bank and finite weights, whatever is in it.
 //
-// Scores and sums are those of 64 bits: which of two is larger decides, and two that differ in the last place of 32 bits are no tie.
+// Scores and sums are those of 64 bits: which of two is larger decides, and two that differ in the last place of 32 bits are no tie.  So that not
+// every expert takes a 64-bit exponential, 32-bit values with known error bounds leave a few candidates, and those are ranked in 64 bits.
 #pragma once
 #include "common.cuh"
 
@@ -25,9 +27,9 @@ __device__ __forceinline__ bool sel_before(double a, int i, double b, int j) { r
 
 __device__ __forceinline__ double sel_sigmoid(double l) { return 1. / (1. + exp(-l)); }
 
-// One row by one warp; E <= 1024, topk <= 31, groups <= 32.  c: E doubles of shared memory of this warp's.
-__device__ __forceinline__ void select_row(const float *row, const float *bias, int E, int topk, const SelRule &rule, double *c, int *picks,
-                                           float *weights, int lane) {
+// One row by one warp in 64 bits throughout: whatever select_row leaves undecided.  c: E doubles of shared memory of this warp's (with a bias).
+__device__ __noinline__ void select_row_slowly(const float *row, const float *bias, int E, int topk, const SelRule &rule, double *c, int *picks,
+                                               float *weights, int lane) {
     const unsigned all = 0xffffffffu;
     double top = 0., z = 1.;                             // softmax: the largest logit, the sum
     if (rule.softmax) {
@@ -48,17 +50,17 @@ __device__ __forceinline__ void select_row(const float *row, const float *bias, 
         if (!rule.softmax) return sel_sigmoid(l);
         return l == -INFINITY ? 0. : l == top ? 1. / z : exp(l - top) / z;
     };
-    for (int e = lane; e < E; e += 32) {
+    auto logit = [&](int e) {
         const float f = row[e];
-        const double l = f == f ? (double)f : -INFINITY;
-        double v = l;
-        if (bias) {
+        return f == f ? (double)f : -INFINITY;
+    };
+    if (bias)
+        for (int e = lane; e < E; e += 32) {
             const float b = bias[e];
-            v = b == b ? score(l) + (double)b : -INFINITY;
+            c[e] = b == b ? score(logit(e)) + (double)b : -INFINITY;
         }
-        c[e] = v;
-    }
     __syncwarp();
+    auto value_of = [&](int e) { return bias ? c[e] : logit(e); };
     unsigned stay = all;
     const int per = E / rule.groups;
     if (rule.keep < rule.groups) {
@@ -66,37 +68,326 @@ __device__ __forceinline__ void select_row(const float *row, const float *bias, 
         if (lane < rule.groups) {
             double first = -INFINITY, second = -INFINITY;
             for (int e = lane * per; e < (lane + 1) * per; ++e) {
-                const double v = c[e];
+                const double v = value_of(e);
                 if (v > first) { second = first; first = v; }
                 else if (v > second) second = v;
             }
-            value = !rule.top2 ? first : bias ? (per > 1 ? first + second : first) : score(first) + (per > 1 ? score(second) : 0.);
+            if (!rule.top2) value = first;
+            else if (!bias) value = score(first) + (per > 1 ? score(second) : 0.);
+            else value = per > 1 && first < INFINITY ? first + second : first;
         }
         int place = 0;
         for (int g = 0; g < rule.groups; ++g) place += sel_before(__shfl_sync(all, value, g), g, value, lane);
         stay = __ballot_sync(all, lane < rule.groups && place < rule.keep);
     }
     unsigned taken = 0;                                  // this lane's e = lane + 32 j
-    double sum = 0.;
-    double mine = 0.;
+    double sum = 0., mine = 0.;
     for (int t = 0; t < topk; ++t) {
         double best = -INFINITY;
         int id = E;
         for (int e = lane, j = 0; e < E; e += 32, ++j)
-            if (!(taken >> j & 1) && (stay >> (e / per) & 1) && (id == E || sel_before(c[e], e, best, id))) { best = c[e]; id = e; }
+            if (!(taken >> j & 1) && (stay >> (e / per) & 1)) {
+                const double v = value_of(e);
+                if (id == E || sel_before(v, e, best, id)) { best = v; id = e; }
+            }
         for (int m = 16; m; m >>= 1) {
             const double ob = __shfl_xor_sync(all, best, m);
             const int oi = __shfl_xor_sync(all, id, m);
             if (oi < E && (id == E || sel_before(ob, oi, best, id))) { best = ob; id = oi; }
         }
         if ((id & 31) == lane) taken |= 1u << (id >> 5);
-        const float f = row[id];
-        const double s = score(f == f ? (double)f : -INFINITY);
+        const double s = score(logit(id));
         sum += s;
         if (lane == t) { mine = s; picks[t] = id; }
     }
     if (lane < topk) weights[lane] = (float)((rule.renorm ? (sum > 0. ? mine / sum : 0.) : mine) * rule.scale);
     if (lane == 0) { picks[topk] = E; weights[topk] = 1.f; }
+}
+
+// 32-bit values as integers of the same order
+__device__ __forceinline__ unsigned sel_ordered(float v) {
+    const unsigned u = __float_as_uint(v + 0.f);          // (-0 is 0)
+    return u ^ ((unsigned)((int)u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float sel_value(unsigned o) { return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o); }
+
+// How far off 32-bit values may be.  A sigmoid (fast exponential, 2 + 1.2 |x| units in the last place, times s (1 - s); fast quotient, 2 units): less
+// than 2^-21.  A softmax score: less than 2^-18 of the largest possible one `most` (its sum: up to 37 additions one after another and the
+// exponentials' own errors; x e^-x stays below 1/2).  c = s + bias by 2^-24 of itself in addition: together, since |bias| <= |c| + s, less than err (2
+// most + |c|).
+__device__ __forceinline__ float sel_err(bool softmax) { return softmax ? 1.f / (1 << 18) : 1.f / (1 << 21); }
+
+// One row by one warp; E <= 1024, topk <= 31, groups <= 32.  c: shared memory of this warp's, for a multiple of 32 experts doubles with a
+// bias, else floats; spot: 32 places.
+//   1. 32-bit c of every expert, in shared memory (in registers the loops over them have to be unrolled: long code, fetched for one pass)
+//   2. groups: 32-bit values by a few lanes a group; those that the error could carry over the border are valued in 64 bits by the whole warp
+//   3. a lower bound of the topk-th largest c: of the lanes' largest values the topk-th; where that leaves more than 32, bisection
+//   4. the candidates, those not provably below it, get a lane each: rank by comparison with all of them, in 64 bits if two are within the error
+// Selection one after another, all in 64 bits (select_row_slowly): 62 us for 8192 rows of 288 experts in 8 groups, 13 us for one row.
+__device__ __forceinline__ void select_row(const float *row, const float *bias, int E, int topk, const SelRule &rule, double *c, int2 *spot, int *picks,
+                                           float *weights, int lane) {
+    const unsigned all = 0xffffffffu;
+    const bool exact = bias == nullptr, grouped = rule.keep < rule.groups;   // exact: the keys are the logits
+    const float err = sel_err(rule.softmax);
+    const int turns = (E + 31) >> 5;
+    float *keys = reinterpret_cast<float *>(c);          // [32 turns], the biases behind them
+    float top = 0.f, z = 1.f, most = 1.f, mine = -INFINITY;                  // most: the largest score there can be;  mine: the lane's largest key
+    bool sound = true;
+    auto clean = [](float l) { return fmaxf(l, -INFINITY); };                // (NaN: -inf)
+    // (fast exponential and reciprocal; 1 / inf is 0, as it should be)
+    auto score = [&](float l) {
+        if (rule.softmax) return __expf(l - top) * most;
+        float r;
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + __expf(-l)));
+        return r;
+    };
+    // every key of this lane by f(key, bias), four on their way at a time
+    auto each = [&](bool biased, auto f) {
+        float *p = keys + lane;
+        int j = 0;
+        for (; j + 4 <= turns; j += 4, p += 128) {
+            float k[4], b[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                k[i] = p[32 * i];
+                b[i] = biased ? p[32 * (turns + i)] : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[32 * i] = f(k[i], b[i]);
+        }
+        for (; j < turns; ++j, p += 32) *p = f(*p, biased ? p[32 * turns] : 0.f);
+    };
+    // All at once to shared memory: through registers the loads of a loop wait for one another (800 clocks for every 32 experts), or the loop is
+    // unrolled.
+    for (int e = lane; e < E; e += 32) {
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(keys + e)), "l"(row + e) : "memory");
+        if (!exact) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(keys + 32 * turns + e)), "l"(bias + e) : "memory");
+    }
+    if (lane + 32 * (turns - 1) >= E) {                  // (behind the last expert)
+        keys[lane + 32 * (turns - 1)] = -INFINITY;
+        if (!exact) keys[lane + 32 * (2 * turns - 1)] = -INFINITY;
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (rule.softmax) {
+        each(false, [&](float l, float) {
+            l = clean(l);
+            mine = fmaxf(mine, l);
+            return l;
+        });
+        top = sel_value(__reduce_max_sync(all, sel_ordered(mine)));
+        z = 0.f;
+        if (top - top == 0.f) {
+            each(false, [&](float l, float) {
+                z += expf(l - top);                      // (exp(-inf) is 0)
+                return l;
+            });
+#pragma unroll
+            for (int m = 16; m; m >>= 1) z += __shfl_xor_sync(all, z, m);
+            most = 1.f / z;
+        } else sound = false;                            // an infinity, or nothing
+    }
+    if (!exact) {
+        mine = -INFINITY;
+        each(true, [&](float l, float b) {
+            l = clean(score(clean(l)) + b);
+            mine = fmaxf(mine, l);
+            return l;
+        });
+    } else if (!rule.softmax) {
+        each(false, [&](float l, float) {
+            l = clean(l);
+            mine = fmaxf(mine, l);
+            return l;
+        });
+    }
+    __syncwarp();
+    if (grouped) {
+        const int per = E / rule.groups, wide = 32 >> (32 - __clz(rule.groups - 1)), g = lane / wide;    // lanes of a group
+        float first = -INFINITY, second = -INFINITY;
+        if (g < rule.groups)
+#pragma unroll 4
+            for (int e = lane - g * wide; e < per; e += wide) {
+                const float v = keys[g * per + e];
+                second = fmaxf(second, fminf(first, v));
+                first = fmaxf(first, v);
+            }
+        for (int m = 1; m < wide; m <<= 1) {
+            const float f = __shfl_xor_sync(all, first, m), s = __shfl_xor_sync(all, second, m);
+            second = fmaxf(fmaxf(second, s), fminf(first, f));
+            first = fmaxf(first, f);
+        }
+        float value = first;
+        if (rule.top2 && exact) value = score(first) + (per > 1 ? score(second) : 0.f);
+        else if (rule.top2 && per > 1 && first < INFINITY) value = first + second;
+        const unsigned o = g < rule.groups ? sel_ordered(value) : 0u;
+        int place = 0;
+        for (int i = 0; i < rule.groups; ++i) {
+            const unsigned other = __shfl_sync(all, o, i * wide);
+            place += other > o || (other == o && i < g);
+        }
+        bool in = g < rule.groups && place < rule.keep;
+        if (!(exact && !rule.top2)) {
+            const float worst = sel_value(__reduce_min_sync(all, in ? o : 0xffffffffu)), best = sel_value(__reduce_max_sync(all, in || g >= rule.groups ? 0u : o));
+            const float apart = 2.2f * err * (4.f * most + fabsf(worst) + fabsf(best));                  // (two sums of two)
+            const bool open_question = g < rule.groups && !(in ? value > best + apart : value < worst - apart);
+            unsigned left = __ballot_sync(all, open_question);
+            if (left && rule.softmax && !exact) sound = false;               // (the sum of the exponentials has 32 bits)
+            else if (left) {
+                const int places = rule.keep - __popc(__ballot_sync(all, in && !open_question && lane == g * wide));
+                double exactly = 0.;
+                for (unsigned todo = left; todo;) {
+                    const int of = (__ffs(todo) - 1) / wide;
+                    todo &= ~(((wide < 32 ? 1u << wide : 0u) - 1u) << of * wide);
+                    double one = -INFINITY, two = -INFINITY;
+                    for (int e = of * per + lane; e < (of + 1) * per; e += 32) {
+                        const float f = row[e];
+                        const double l = f == f ? (double)f : -INFINITY;
+                        double v;
+                        if (exact) v = l;
+                        else {
+                            const float b = bias[e];
+                            v = b == b ? sel_sigmoid(l) + (double)b : -INFINITY;
+                        }
+                        if (v > one) { two = one; one = v; }
+                        else if (v > two) two = v;
+                    }
+                    for (int m = 16; m; m >>= 1) {
+                        const double f = __shfl_xor_sync(all, one, m), t = __shfl_xor_sync(all, two, m);
+                        two = fmax(fmax(two, t), fmin(one, f));
+                        one = fmax(one, f);
+                    }
+                    // (without a bias the sum is one of scores: of a softmax those times its sum, for all groups alike)
+                    auto score64 = [&](double l) { return rule.softmax ? exp(l - (double)top) : sel_sigmoid(l); };
+                    const double sum = !rule.top2 ? one : exact ? score64(one) + (per > 1 ? score64(two) : 0.) : per > 1 && one < INFINITY ? one + two : one;
+                    if (g == of) exactly = sum;
+                }
+                int before = 0;
+                for (int i = 0; i < rule.groups; ++i) {
+                    const double other = __shfl_sync(all, exactly, i * wide);
+                    before += (left >> i * wide & 1) && sel_before(other, i, exactly, g);
+                }
+                if (open_question) in = before < places;
+            }
+        }
+        // experts of the other groups: NaN, which no comparison finds
+        const unsigned stay = __ballot_sync(all, in);
+        mine = -INFINITY;
+        float at = (float)lane + 0.5f;
+        const float groups_per_expert = 1.f / (float)per;
+        each(false, [&](float k, float) {
+            const int of = (int)(at * groups_per_expert);
+            at += 32.f;
+            if (!(stay >> (of * wide & 31) & 1)) k = NAN;
+            mine = fmaxf(mine, k);
+            return k;
+        });
+    }
+    // of the lanes' largest keys the topk-th
+    unsigned bound = 0, rest = sel_ordered(mine);
+    const unsigned highest = __reduce_max_sync(all, rest);
+    for (int t = 0; t < topk; ++t) {
+        bound = __reduce_max_sync(all, rest);
+        const unsigned same = __ballot_sync(all, rest == bound);
+        if (lane == __ffs(same) - 1) rest = 0;
+    }
+    auto threshold = [&](unsigned o) {
+        const float t = sel_value(o);
+        return exact || t - t != 0.f ? t : t - 2.5f * err * (2.f * most + fabsf(t));
+    };
+    // which keys of the lane are that large, a bit a turn
+    auto marked = [&](float from) {
+        unsigned mask = 0;
+#pragma unroll 4
+        for (int j = 0; j < turns; ++j) mask |= (unsigned)(keys[32 * j + lane] >= from) << j;
+        if (lane + 32 * (turns - 1) >= E) mask &= ~(1u << (turns - 1));
+        return mask;
+    };
+    auto count = [&](float from) { return (int)__reduce_add_sync(all, __popc(marked(from))); };
+    unsigned mask = marked(threshold(bound));
+    int n = (int)__reduce_add_sync(all, __popc(mask));
+    if (n > 32) {                                        // (bound: at least topk are that large;  above: fewer)
+        unsigned above = highest + 1;
+        while (n > 32 && above - bound > 1) {
+            const unsigned middle = bound + ((above - bound) >> 1);
+            if (count(sel_value(middle)) >= topk) {
+                bound = middle;
+                n = count(threshold(bound));
+            } else above = middle;
+        }
+        mask = marked(threshold(bound));
+        if (n > 32 && exact) {                           // ties: the lowest ids of those at the bound
+            mask = marked(sel_value(bound + 1));
+            int left = topk - (int)__reduce_add_sync(all, __popc(mask));
+            for (int j = 0; j < turns; ++j) {
+                const unsigned same = __ballot_sync(all, lane + 32 * j < E && keys[32 * j + lane] == sel_value(bound));
+                if ((same >> lane & 1) && __popc(same & ((1u << lane) - 1)) < left) mask |= 1u << j;
+                left = max(left - __popc(same), 0);
+            }
+            n = topk;
+        }
+    }
+    if (n <= 32) {                                       // a place for each
+        int at = __popc(mask);
+#pragma unroll
+        for (int m = 1; m < 32; m <<= 1) {
+            const int below = __shfl_up_sync(all, at, m);
+            if (lane >= m) at += below;
+        }
+        at -= __popc(mask);
+        for (; mask; mask &= mask - 1, ++at) {
+            const int e = 32 * (__ffs(mask) - 1) + lane;
+            spot[at] = make_int2(e, __float_as_int(keys[e]));
+        }
+    }
+    if (n > 32) sound = false;                           // (ties within the error)
+    if (sound) {
+        __syncwarp();
+        const bool live = lane < n;
+        const int2 candidate = live ? spot[lane] : make_int2(E, 0);
+        const int id = candidate.x;
+        const float k32 = live ? __int_as_float(candidate.y) : -INFINITY, l = live ? clean(row[id]) : 0.f, apart = 2.f * err * (2.f * most + fabsf(k32));
+        int rank = 0;
+        bool close = false;
+#pragma unroll 4
+        for (int i = 0; i < n; ++i) {
+            const float other = __shfl_sync(all, k32, i);
+            const int oi = __shfl_sync(all, id, i);
+            rank += other > k32 || (other == k32 && oi < id);
+            close |= oi != id && !(fabsf(other - k32) > apart);
+        }
+        const float s = rule.softmax ? expf(l - top) * most : 1.f / (1.f + expf(-l));
+        if (!exact && __any_sync(all, live && close)) {  // in 64 bits
+            double s64 = 0., v = -INFINITY;
+            if (live) {
+                s64 = rule.softmax ? exp((double)l - (double)top) / (double)z : sel_sigmoid(l);
+                const float b = bias[id];
+                v = b == b ? s64 + (double)b : -INFINITY;
+            }
+            rank = 0;
+            for (int i = 0; i < n; ++i) {
+                const double ov = __shfl_sync(all, v, i), os = __shfl_sync(all, s64, i);
+                const int oi = __shfl_sync(all, id, i);
+                rank += sel_before(ov, oi, v, id);
+                // (the sum of a softmax has 32 bits: it scales all scores alike)
+                if (rule.softmax && live && os != s64 && fabs(ov - v) <= 2. * err * fabs(os - s64)) sound = false;
+            }
+        }
+        const bool chosen = live && rank < topk;
+        float sum = chosen ? s : 0.f;
+#pragma unroll
+        for (int m = 16; m; m >>= 1) sum += __shfl_xor_sync(all, sum, m);
+        if (rule.renorm && sum < 1e-20f) sound = false;  // (scores that 32 bits hold badly, or not at all)
+        if (__all_sync(all, sound)) {
+            if (chosen) {
+                picks[rank] = id;
+                weights[rank] = (rule.renorm ? s / sum : s) * rule.scale;
+            }
+            if (lane == 0) { picks[topk] = E; weights[topk] = 1.f; }
+            return;
+        }
+    }
+    __syncwarp();
+    select_row_slowly(row, bias, E, topk, rule, c, picks, weights, lane);
 }
 
 }  // namespace gf

@@ -303,7 +303,7 @@ int glmflash_route(void *stream, const uint16_t *x, int x_stride, const uint16_t
  *   s = 1 / (1 + exp(-l))  or  exp(l - max) / sum exp(l - max) over all experts
  *   c = s + bias (-inf where the bias is NaN); without a bias c = l, whose order is that of the scores
  *   groups of experts / groups neighbouring ids: a group's value is its largest c, or the sum of its two largest c (without a
- *     bias: s); the keep_groups largest stay, ties to the lower group
+ *     bias: s; +inf where one is); the keep_groups largest stay, ties to the lower group
  *   picks = the topk largest c of the groups that stay, descending, ties to the lower id
  *   weight = s * scale, or with renorm s / (sum of the chosen s) * scale, 0 where that sum is 0
  * The order is that of s and c in 64 bits (values that 32 bits cannot tell apart are no tie); weights are computed in fp32 or more.
