@@ -582,11 +582,12 @@ _calls = None
 
 
 def _hot():
-    """(current device, current raw stream, topk_by, route_by, linear): looked up once, since a small call's lookups cost as much as its kernel."""
+    """Current device, current raw stream, the three calls, three types: looked up once, since a small call's lookups cost as much as its kernel."""
     global _calls
     if _calls is None:
-        c, L = _torch()._C, lib()
-        _calls = c._cuda_getDevice, c._cuda_getCurrentRawStream, L.glmflash_topk_by, L.glmflash_route_by, L.glmflash_linear
+        torch, L = _torch(), lib()
+        _calls = (torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream, L.glmflash_topk_by, L.glmflash_route_by, L.glmflash_linear,
+                  torch.float32, torch.int32, torch.bfloat16)
     return _calls
 
 
@@ -609,15 +610,7 @@ def _table_refusal(logits, picks, weights, bias, dev):
     _require(picks.is_contiguous() and weights.is_contiguous(), "picks and weights must be contiguous")
     _require(bias is None or (bias.dtype is torch.float32 and bias.shape == (E,) and bias.get_device() == dev and bias.is_contiguous()),
              "bias must be float32 [experts], contiguous, on the same device")
-    raise GlmFlashError("logits must have neighbouring experts side by side")
-
-
-def _table_fits(logits, picks, weights, bias, dev):
-    f32, shape, table = _cuda_torch.float32, logits.shape, picks.shape
-    return (logits.dtype is f32 and weights.dtype is f32 and picks.dtype is _cuda_torch.int32 and len(shape) == 2 and len(table) == 2 and
-            weights.shape == table and table[0] == shape[0] and logits.get_device() == dev and picks.get_device() == dev and
-            weights.get_device() == dev and picks.is_contiguous() and weights.is_contiguous() and
-            (bias is None or (bias.dtype is f32 and bias.shape == shape[1:] and bias.get_device() == dev and bias.is_contiguous())))
+    raise GlmFlashError("logits must have neighbouring experts side by side (route_by: be contiguous)")
 
 
 def topk_by(logits, picks, weights, bias=None, scores="sigmoid", groups=1, keep_groups=None, group_score="max", renorm=True, scale=1.0,
@@ -625,42 +618,57 @@ def topk_by(logits, picks, weights, bias=None, scores="sigmoid", groups=1, keep_
     """Routing table of logits fp32 [rows][E] by a rule (glmflash_topk_by): `scores` "sigmoid" or "softmax", `bias` fp32 [E] added to them
     for the choice alone, `groups` of neighbouring experts of which the `keep_groups` best by `group_score` ("max" or "top2") stay, weights
     renormalised or not and times `scale`.  Writes picks int32 / weights fp32 [rows][k + 1] (shared expert last) and returns them."""
-    get_device, get_stream, call, _, _ = _calls or _hot()
-    dev = get_device()
-    if not _table_fits(logits, picks, weights, bias, dev):
+    get_device, get_stream, call, _, _, f32, i32, _ = _calls or _hot()
+    dev, shape, table = get_device(), logits.shape, picks.shape
+    if len(shape) != 2 or len(table) != 2:
         _table_refusal(logits, picks, weights, bias, dev)
-    rows, E = logits.shape
-    step, side = logits.stride()
-    if side != 1 and E > 1:
+    (rows, E), (step, side) = shape, logits.stride()
+    if not (logits.dtype is f32 and weights.dtype is f32 and picks.dtype is i32 and weights.shape == table and table[0] == rows and
+            logits.get_device() == picks.get_device() == weights.get_device() == dev and picks.is_contiguous() and weights.is_contiguous() and
+            (side == 1 or E == 1)):
         _table_refusal(logits, picks, weights, bias, dev)
-    if call(get_stream(dev) if stream is None else stream.cuda_stream, logits.data_ptr(), step if rows > 1 else E, None if bias is None else bias.data_ptr(),
-            rows, E, picks.shape[1] - 1, _rule(scores, groups, keep_groups, group_score, renorm, scale), _RULE.size, picks.data_ptr(), weights.data_ptr(), pdl):
+    if bias is None:
+        bp = None
+    else:
+        if not (bias.dtype is f32 and bias.shape == shape[1:] and bias.get_device() == dev and bias.is_contiguous()):
+            _table_refusal(logits, picks, weights, bias, dev)
+        bp = bias.data_ptr()
+    if call(get_stream(dev) if stream is None else stream.cuda_stream, logits.data_ptr(), step if rows > 1 else E, bp, rows, E, table[1] - 1,
+            _rule(scores, groups, keep_groups, group_score, renorm, scale), 32, picks.data_ptr(), weights.data_ptr(), pdl):
         _check(-1)
     return picks, weights
 
 
 def route_by(x, wr, logits, picks, weights, bias=None, scores="sigmoid", groups=1, keep_groups=None, group_score="max", renorm=True,
              scale=1.0, stream=None, pdl=1):
-    """router_logits + topk_by: x bf16 [rows][hidden], wr bf16 [E][hidden]; fills logits, picks and weights."""
-    get_device, get_stream, _, call, _ = _calls or _hot()
-    dev, bf16 = get_device(), _cuda_torch.bfloat16
-    if not (_table_fits(logits, picks, weights, bias, dev) and logits.is_contiguous()):
-        _require(logits.is_contiguous(), "logits must be contiguous")
+    """The router product and topk_by in one call: x bf16 [rows][hidden], wr bf16 [E][hidden]; fills logits, picks and weights."""
+    get_device, get_stream, _, call, _, f32, i32, bf16 = _calls or _hot()
+    dev, shape, table, xshape = get_device(), logits.shape, picks.shape, x.shape
+    if len(shape) != 2 or len(table) != 2:
         _table_refusal(logits, picks, weights, bias, dev)
-    (rows, E), xshape, wshape = logits.shape, x.shape, wr.shape
-    if not (len(xshape) == 2 and xshape[0] == rows and wshape == (E, xshape[1])):
+    rows, E = shape
+    if not (logits.dtype is f32 and weights.dtype is f32 and picks.dtype is i32 and weights.shape == table and table[0] == rows and
+            logits.get_device() == picks.get_device() == weights.get_device() == dev and picks.is_contiguous() and weights.is_contiguous() and
+            logits.is_contiguous()):
+        _table_refusal(logits, picks, weights, bias, dev)
+    if bias is None:
+        bp = None
+    else:
+        if not (bias.dtype is f32 and bias.shape == shape[1:] and bias.get_device() == dev and bias.is_contiguous()):
+            _table_refusal(logits, picks, weights, bias, dev)
+        bp = bias.data_ptr()
+    if not (len(xshape) == 2 and xshape[0] == rows and wr.shape == (E, xshape[1])):
         raise GlmFlashError("x must be [rows][hidden] and the router matrix [experts][hidden]")
-    if x.dtype is not bf16 or wr.dtype is not bf16:
+    if not (x.dtype is wr.dtype is bf16):
         raise GlmFlashError("x and the router matrix must be bfloat16")
-    if x.get_device() != dev or wr.get_device() != dev:
+    if not (x.get_device() == wr.get_device() == dev):
         raise GlmFlashError("tensors must be on one device")
     step, side = x.stride()
     H = xshape[1]
     if not (side == 1 or H == 1) or not wr.is_contiguous():
         raise GlmFlashError("rows of x and the router matrix must be contiguous")
-    if call(get_stream(dev) if stream is None else stream.cuda_stream, x.data_ptr(), step if rows > 1 else H, wr.data_ptr(),
-            None if bias is None else bias.data_ptr(), rows, H, E, picks.shape[1] - 1, _rule(scores, groups, keep_groups, group_score, renorm, scale),
-            _RULE.size, logits.data_ptr(), picks.data_ptr(), weights.data_ptr(), pdl):
+    if call(get_stream(dev) if stream is None else stream.cuda_stream, x.data_ptr(), step if rows > 1 else H, wr.data_ptr(), bp, rows, H, E, table[1] - 1,
+            _rule(scores, groups, keep_groups, group_score, renorm, scale), 32, logits.data_ptr(), picks.data_ptr(), weights.data_ptr(), pdl):
         _check(-1)
     return picks, weights
 
@@ -708,7 +716,7 @@ def _operands(x, w, w_up, dev):
 
 
 def _dense(x, w, w_up, out, bias, bias_up, act, residual, out_dtype, limit, stream, pdl):
-    get_device, get_stream, _, _, call = _calls or _hot()
+    get_device, get_stream, _, _, call, _, _, _ = _calls or _hot()
     codes = _TYPE_CODES or _type_codes()
     dt, dev, xshape, wshape = x.dtype, get_device(), x.shape, w.shape
     code = codes.get(dt, 0)

@@ -352,8 +352,23 @@ extern "C" int glmflash_route_by(void *stream, const uint16_t *x, int64_t x_stri
     SelRule sel;
     if (check_rule(rule, rule_bytes, experts, topk, &sel)) return -1;
     GF_REQUIRE(rows > 0 && hidden > 0 && hidden % 8 == 0, "rows positive; hidden a multiple of 8");
-    GF_REQUIRE(x_stride >= hidden && x_stride % 8 == 0 && x_stride <= INT32_MAX, "x_stride must be >= hidden and a multiple of 8");
+    GF_REQUIRE(x_stride >= hidden && x_stride % 8 == 0, "x_stride must be >= hidden and a multiple of 8");
     GF_REQUIRE(((uintptr_t)x | (uintptr_t)wr) % 16 == 0, "x and the router matrix must be 16-byte aligned");
-    if (launch_route((cudaStream_t)stream, x, (int)x_stride, wr, rows, hidden, experts, 0, logits, nullptr, nullptr, pdl != 0)) return -1;
+    // The dense products, whose kernels are faster than route_kernel for any number of rows and experts (us, logits alone: 2048 x 64 experts, 1 row 2.7
+    // | 3.5, 4096 rows 8.3 | 9.5; 4096 x 288, 1 row 3.7 | 18.4, 4096 rows 18.4 | 72.3), and the selection behind them.
+    glmflash_linear_args a = {};
+    a.x = x;
+    a.w = wr;
+    a.out = logits;
+    a.x_stride = x_stride;
+    a.w_stride = hidden;
+    a.out_stride = experts;
+    a.rows = rows;
+    a.inner = hidden;
+    a.outer = experts;
+    a.type = GLMFLASH_BF16;
+    a.out_type = GLMFLASH_F32;
+    a.pdl = pdl;
+    if (glmflash_linear(stream, &a, sizeof(a))) return -1;
     return launch_select((cudaStream_t)stream, logits, experts, bias, rows, experts, topk, sel, picks, weights, pdl != 0);
 }

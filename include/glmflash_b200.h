@@ -326,8 +326,8 @@ size_t glmflash_topk_rule_bytes(void);
  * fp32 [rows][topk + 1].  rule: host memory, read during the call.  Enqueues work only (graph-capturable); pdl as above. */
 int glmflash_topk_by(void *stream, const float *logits, int64_t logits_stride, const float *bias, int rows, int experts, int topk,
                      const glmflash_topk_rule *rule, size_t rule_bytes, int32_t *picks, float *weights, int pdl);
-/* The router product (glmflash_router_logits) and the selection from the logits that it leaves in `logits` (fp32 [rows][experts]):
- * the bytes of the two calls one after the other. */
+/* The router product and the selection: `logits` (fp32 [rows][experts], caller's) receives the product (the bytes of glmflash_linear
+ * with an fp32 output), picks and weights are glmflash_topk_by's of it.  x bf16 [rows][x_stride], wr bf16 [experts][hidden]. */
 int glmflash_route_by(void *stream, const uint16_t *x, int64_t x_stride, const uint16_t *wr, const float *bias, int rows, int hidden,
                       int experts, int topk, const glmflash_topk_rule *rule, size_t rule_bytes, float *logits, int32_t *picks,
                       float *weights, int pdl);

@@ -206,7 +206,7 @@ def test_strided_logits_a_stream_and_replay(pkg, cuda):
     (1, 2048, 64, 4, dict(scale=2.5)), (16, 4096, 288, 8, dict(groups=8, keep_groups=4, group_score="top2")), (300, 256, 65, 3, dict(scores="softmax")),
     (2500, 512, 128, 8, dict(scores="softmax", renorm=False)), (5, 264, 1024, 31, {}), (17, 8, 1, 1, {}), (4000, 128, 32, 4, dict(groups=4, keep_groups=2))])
 def test_route_by_is_logits_and_selection(pkg, cuda, rows, H, E, k, rule):
-    """The bytes of router_logits followed by topk_by on the same rows."""
+    """The bytes of the dense product in fp32 followed by topk_by on the same rows."""
     import torch
     gen = torch.Generator(device=cuda).manual_seed(rows)
     x = torch.randn((rows, H + 8), generator=gen, device=cuda).to(torch.bfloat16)[:, :H]
@@ -216,8 +216,7 @@ def test_route_by_is_logits_and_selection(pkg, cuda, rows, H, E, k, rule):
         x[1], x[2, 0], x[3, 3] = 0, float("nan"), float("inf")
     out = [torch.full((rows, E), 9.0, device=cuda), torch.full((rows, k + 1), -7, dtype=torch.int32, device=cuda), torch.zeros((rows, k + 1), device=cuda)]
     pkg.route_by(x, wr, *out, bias=bias, **rule)
-    l2 = torch.empty_like(out[0])
-    pkg.router_logits(x, wr, l2)
+    l2 = pkg.linear(x, wr, out_dtype=torch.float32)
     p2, w2 = torch.empty_like(out[1]), torch.empty_like(out[2])
     pkg.topk_by(l2, p2, w2, bias=bias, **rule)
     torch.cuda.synchronize()
