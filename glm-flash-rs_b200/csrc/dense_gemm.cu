@@ -162,6 +162,7 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
                         at.next(depth);
                     }
                 }
+            if (!ok) t5_settle();
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(DW_REGS_EPI));
@@ -366,6 +367,7 @@ dense_thin_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
             ++in_chain;
             at.next(d.depth);
         }
+        if (!ok) t5_settle();
     } else if (warp >= 4) {
         pdl_wait();
         asm volatile("barrier.sync 1, 288;" ::: "memory");
@@ -543,7 +545,9 @@ int dense_gemm(cudaStream_t s, const DenseArgs &a, bool pdl) {
     if (thin < wide) {
         if (dense_maps(&maps, a, h.t, copies)) return -1;
         const int bytes = mats * DW_A + h.t * DW_K * 2, parts = cluster * h.slots * mats * 2048;
-        const size_t smem = 1024 + (h.alias ? std::max(h.depth * bytes, parts) : h.depth * bytes + parts);
+        // At least the share of the shared memory that it takes of the tensor memory: CTAs that fit on an SM side by side (of two streams) then never
+        // wait for each other's tensor memory, which CTAs of two clusters could do crosswise, and for good.
+        const size_t smem = std::max<size_t>(1024 + (h.alias ? std::max(h.depth * bytes, parts) : h.depth * bytes + parts), (size_t)DT_SMEM * h.cols / 512);
         return launch_kc(mats == 2 ? dense_thin_kernel<2> : dense_thin_kernel<1>, dim3((unsigned)(across * h.row_tiles * cluster)), dim3(DT_THREADS),
                          dim3((unsigned)cluster), smem, s, pdl, maps, a, h);
     }

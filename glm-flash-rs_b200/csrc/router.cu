@@ -243,23 +243,26 @@ __global__ void __launch_bounds__(256) route_kernel(const __nv_bfloat16 *__restr
     if (cn > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
 
+// (CTAs that stay and take row after row, the biases kept and the next row on its way, were slower: 18.3 against 14.7 us for 8192 rows of 288 experts in
+// 8 groups.  What bounds it is the chain of a row, which other rows' hide.)
 constexpr int SEL_WARPS = 4;
 __global__ void __launch_bounds__(SEL_WARPS * 32, 8) select_kernel(const float *logits, int64_t stride, const float *bias, int rows, int E, int topk, SelRule rule,
                                                                    int *picks, float *weights) {
     extern __shared__ double sel_values[];
     __shared__ int2 spot[SEL_WARPS][32];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.x * SEL_WARPS + warp;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t r = (int64_t)blockIdx.x * SEL_WARPS + warp;
     pdl_wait();
     pdl_launch_dependents();
     if (r >= rows) return;
-    select_row(logits + r * stride, bias, E, topk, rule, sel_values + warp * (bias ? (E + 31) / 32 * 32 : (E + 31) / 32 * 16), spot[warp],
-               picks + (size_t)r * (topk + 1), weights + (size_t)r * (topk + 1), lane);
+    select_row(logits + r * stride, bias, E, topk, rule, reinterpret_cast<float *>(sel_values) + warp * ((E + 31) / 32 * (bias ? 64 : 32)), spot[warp],
+               picks + r * (topk + 1), weights + r * (topk + 1), lane);
 }
 
 static int launch_select(cudaStream_t s, const float *logits, int64_t stride, const float *bias, int rows, int E, int topk, const SelRule &rule, int *picks,
                          float *weights, bool pdl) {
-    const dim3 grid((unsigned)((rows + SEL_WARPS - 1) / SEL_WARPS)), block(SEL_WARPS * 32);
-    const size_t smem = (size_t)SEL_WARPS * ((E + 31) / 32 * 32) * (bias ? sizeof(double) : sizeof(float));
+    const dim3 grid((unsigned)(((int64_t)rows + SEL_WARPS - 1) / SEL_WARPS)), block(SEL_WARPS * 32);
+    const size_t smem = (size_t)SEL_WARPS * ((E + 31) / 32 * 32) * (bias ? 2 : 1) * sizeof(float);
     return launch_k(select_kernel, grid, block, smem, s, pdl, logits, stride, bias, rows, E, topk, rule, picks, weights);
 }
 

@@ -117,20 +117,85 @@ __device__ __forceinline__ float sel_value(unsigned o) { return __uint_as_float(
 // most + |c|).
 __device__ __forceinline__ float sel_err(bool softmax) { return softmax ? 1.f / (1 << 18) : 1.f / (1 << 21); }
 
-// One row by one warp; E <= 1024, topk <= 31, groups <= 32.  c: shared memory of this warp's, for a multiple of 32 experts doubles with a
-// bias, else floats; spot: 32 places.
+// What few rows need, kept out of the others' way (registers):
+// the sum of a softmax
+__device__ __forceinline__ double sel_sum(const float *row, int E, float top, int lane) {
+    double sum = 0.;
+    for (int e = lane; e < E; e += 32) sum += exp((double)fmaxf(row[e], -INFINITY) - (double)top);
+    for (int m = 16; m; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+    return sum;
+}
+// of the groups in `left` (the bits of their lanes, `wide` a group) how many come before this lane's, by their values in 64 bits
+__device__ __noinline__ int sel_groups_before(const float *row, const float *bias, int E, const SelRule &rule, float top, unsigned left, int wide, int lane) {
+    const unsigned all = 0xffffffffu;
+    const int per = E / rule.groups, g = lane / wide;
+    // (without a bias a softmax's sum is left out: it scales all alike)
+    const double sum64 = rule.softmax && bias ? sel_sum(row, E, top, lane) : 1.;
+    auto score = [&](double l) { return rule.softmax ? exp(l - (double)top) / sum64 : sel_sigmoid(l); };
+    double value = 0.;
+    for (unsigned todo = left; todo;) {
+        const int of = (__ffs(todo) - 1) / wide;
+        todo &= ~(((1u << wide) - 1u) << of * wide);     // (two groups at least: wide <= 16)
+        double one = -INFINITY, two = -INFINITY;
+        for (int e = of * per + lane; e < (of + 1) * per; e += 32) {
+            const double l = fmaxf(row[e], -INFINITY);
+            double v = l;
+            if (bias) {
+                const float b = bias[e];
+                v = b == b ? score(l) + (double)b : -INFINITY;
+            }
+            if (v > one) { two = one; one = v; }
+            else if (v > two) two = v;
+        }
+        for (int m = 16; m; m >>= 1) {
+            const double f = __shfl_xor_sync(all, one, m), t = __shfl_xor_sync(all, two, m);
+            two = fmax(fmax(two, t), fmin(one, f));
+            one = fmax(one, f);
+        }
+        const double sum = !rule.top2 ? one : !bias ? score(one) + (per > 1 ? score(two) : 0.) : per > 1 && one < INFINITY ? one + two : one;
+        if (g == of) value = sum;
+    }
+    int before = 0;
+    for (int i = 0; i < rule.groups; ++i) {
+        const double other = __shfl_sync(all, value, i * wide);
+        before += (left >> i * wide & 1) && sel_before(other, i, value, g);
+    }
+    return before;
+}
+// rank of this lane's candidate (logit l, bias b) among n by c in 64 bits
+__device__ __noinline__ int sel_rank(const float *row, int E, int softmax, float top, bool live, float l, float b, int id, int n, int lane) {
+    const double sum64 = softmax ? sel_sum(row, E, top, lane) : 1.;
+    double v = -INFINITY;
+    if (live && b == b) v = (softmax ? exp((double)l - (double)top) / sum64 : sel_sigmoid(l)) + (double)b;
+    int rank = 0;
+    for (int i = 0; i < n; ++i) rank += sel_before(__shfl_sync(0xffffffffu, v, i), __shfl_sync(0xffffffffu, id, i), v, id);
+    return rank;
+}
+
+// E values to shared memory, in flight on return.  All at once: through registers the loads of a loop wait for one
+// another (800 clocks for every 32 experts), or the loop is unrolled.
+__device__ __forceinline__ void sel_fetch(float *to, const float *from, int E, int lane) {
+    const uint32_t at = smem_u32(to);
+    if (((uintptr_t)from | E * 4) % 16 == 0)
+        for (int e = 4 * lane; e < E; e += 128) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + 4 * e), "l"(from + e) : "memory");
+    else
+        for (int e = lane; e < E; e += 32) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(at + 4 * e), "l"(from + e) : "memory");
+}
+
+// One row by one warp; E <= 1024, topk <= 31, groups <= 32.  keys: shared memory of this warp's, a multiple of 32 experts floats, as many again behind
+// them with a bias; spot: 32 places.
 //   1. 32-bit c of every expert, in shared memory (in registers the loops over them have to be unrolled: long code, fetched for one pass)
 //   2. groups: 32-bit values by a few lanes a group; those that the error could carry over the border are valued in 64 bits by the whole warp
-//   3. a lower bound of the topk-th largest c: of the lanes' largest values the topk-th; where that leaves more than 32, bisection
+//   3. a lower bound of the topk-th largest c: of the largest values of the lanes' shares the topk-th; where that leaves more than 32, bisection
 //   4. the candidates, those not provably below it, get a lane each: rank by comparison with all of them, in 64 bits if two are within the error
 // Selection one after another, all in 64 bits (select_row_slowly): 62 us for 8192 rows of 288 experts in 8 groups, 13 us for one row.
-__device__ __forceinline__ void select_row(const float *row, const float *bias, int E, int topk, const SelRule &rule, double *c, int2 *spot, int *picks,
+__device__ __forceinline__ void select_row(const float *row, const float *bias, int E, int topk, const SelRule &rule, float *keys, int2 *spot, int *picks,
                                            float *weights, int lane) {
     const unsigned all = 0xffffffffu;
     const bool exact = bias == nullptr, grouped = rule.keep < rule.groups;   // exact: the keys are the logits
     const float err = sel_err(rule.softmax);
     const int turns = (E + 31) >> 5;
-    float *keys = reinterpret_cast<float *>(c);          // [32 turns], the biases behind them
+    float *biases = keys + 32 * turns;
     float top = 0.f, z = 1.f, most = 1.f, mine = -INFINITY;                  // most: the largest score there can be;  mine: the lane's largest key
     bool sound = true;
     auto clean = [](float l) { return fmaxf(l, -INFINITY); };                // (NaN: -inf)
@@ -144,30 +209,28 @@ __device__ __forceinline__ void select_row(const float *row, const float *bias, 
     // every key of this lane by f(key, bias), four on their way at a time
     auto each = [&](bool biased, auto f) {
         float *p = keys + lane;
+        const float *q = biases + lane;
         int j = 0;
-        for (; j + 4 <= turns; j += 4, p += 128) {
+        for (; j + 4 <= turns; j += 4, p += 128, q += 128) {
             float k[4], b[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 k[i] = p[32 * i];
-                b[i] = biased ? p[32 * (turns + i)] : 0.f;
+                b[i] = biased ? q[32 * i] : 0.f;
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) p[32 * i] = f(k[i], b[i]);
         }
-        for (; j < turns; ++j, p += 32) *p = f(*p, biased ? p[32 * turns] : 0.f);
+        for (; j < turns; ++j, p += 32, q += 32) *p = f(*p, biased ? *q : 0.f);
     };
-    // All at once to shared memory: through registers the loads of a loop wait for one another (800 clocks for every 32 experts), or the loop is
-    // unrolled.
-    for (int e = lane; e < E; e += 32) {
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(keys + e)), "l"(row + e) : "memory");
-        if (!exact) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(keys + 32 * turns + e)), "l"(bias + e) : "memory");
-    }
+    sel_fetch(keys, row, E, lane);
+    if (!exact) sel_fetch(biases, bias, E, lane);
     if (lane + 32 * (turns - 1) >= E) {                  // (behind the last expert)
         keys[lane + 32 * (turns - 1)] = -INFINITY;
-        if (!exact) keys[lane + 32 * (2 * turns - 1)] = -INFINITY;
+        if (!exact) biases[lane + 32 * (turns - 1)] = -INFINITY;
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncwarp();
     if (rule.softmax) {
         each(false, [&](float l, float) {
             l = clean(l);
@@ -211,6 +274,7 @@ __device__ __forceinline__ void select_row(const float *row, const float *bias, 
                 second = fmaxf(second, fminf(first, v));
                 first = fmaxf(first, v);
             }
+        const float own = first;
         for (int m = 1; m < wide; m <<= 1) {
             const float f = __shfl_xor_sync(all, first, m), s = __shfl_xor_sync(all, second, m);
             second = fmaxf(fmaxf(second, s), fminf(first, f));
@@ -231,56 +295,21 @@ __device__ __forceinline__ void select_row(const float *row, const float *bias, 
             const float apart = 2.2f * err * (4.f * most + fabsf(worst) + fabsf(best));                  // (two sums of two)
             const bool open_question = g < rule.groups && !(in ? value > best + apart : value < worst - apart);
             unsigned left = __ballot_sync(all, open_question);
-            if (left && rule.softmax && !exact) sound = false;               // (the sum of the exponentials has 32 bits)
-            else if (left) {
+            if (left && sound) {
                 const int places = rule.keep - __popc(__ballot_sync(all, in && !open_question && lane == g * wide));
-                double exactly = 0.;
-                for (unsigned todo = left; todo;) {
-                    const int of = (__ffs(todo) - 1) / wide;
-                    todo &= ~(((wide < 32 ? 1u << wide : 0u) - 1u) << of * wide);
-                    double one = -INFINITY, two = -INFINITY;
-                    for (int e = of * per + lane; e < (of + 1) * per; e += 32) {
-                        const float f = row[e];
-                        const double l = f == f ? (double)f : -INFINITY;
-                        double v;
-                        if (exact) v = l;
-                        else {
-                            const float b = bias[e];
-                            v = b == b ? sel_sigmoid(l) + (double)b : -INFINITY;
-                        }
-                        if (v > one) { two = one; one = v; }
-                        else if (v > two) two = v;
-                    }
-                    for (int m = 16; m; m >>= 1) {
-                        const double f = __shfl_xor_sync(all, one, m), t = __shfl_xor_sync(all, two, m);
-                        two = fmax(fmax(two, t), fmin(one, f));
-                        one = fmax(one, f);
-                    }
-                    // (without a bias the sum is one of scores: of a softmax those times its sum, for all groups alike)
-                    auto score64 = [&](double l) { return rule.softmax ? exp(l - (double)top) : sel_sigmoid(l); };
-                    const double sum = !rule.top2 ? one : exact ? score64(one) + (per > 1 ? score64(two) : 0.) : per > 1 && one < INFINITY ? one + two : one;
-                    if (g == of) exactly = sum;
-                }
-                int before = 0;
-                for (int i = 0; i < rule.groups; ++i) {
-                    const double other = __shfl_sync(all, exactly, i * wide);
-                    before += (left >> i * wide & 1) && sel_before(other, i, exactly, g);
-                }
+                const int before = sel_groups_before(row, bias, E, rule, top, left, wide, lane);
                 if (open_question) in = before < places;
             }
         }
         // experts of the other groups: NaN, which no comparison finds
-        const unsigned stay = __ballot_sync(all, in);
-        mine = -INFINITY;
-        float at = (float)lane + 0.5f;
-        const float groups_per_expert = 1.f / (float)per;
-        each(false, [&](float k, float) {
-            const int of = (int)(at * groups_per_expert);
-            at += 32.f;
-            if (!(stay >> (of * wide & 31) & 1)) k = NAN;
-            mine = fmaxf(mine, k);
-            return k;
-        });
+        if (g < rule.groups && !in)
+            for (int e = lane - g * wide; e < per; e += wide) keys[g * per + e] = NAN;
+        __syncwarp();
+        if (rule.keep * wide >= topk) mine = in ? own : -INFINITY;           // a lane's share of its group
+        else {                                                               // too few lanes: every 32nd expert as before
+            mine = -INFINITY;
+            for (int e = lane; e < E; e += 32) mine = fmaxf(mine, keys[e]);
+        }
     }
     // of the lanes' largest keys the topk-th
     unsigned bound = 0, rest = sel_ordered(mine);
@@ -350,27 +379,15 @@ __device__ __forceinline__ void select_row(const float *row, const float *bias, 
         bool close = false;
 #pragma unroll 4
         for (int i = 0; i < n; ++i) {
-            const float other = __shfl_sync(all, k32, i);
-            const int oi = __shfl_sync(all, id, i);
-            rank += other > k32 || (other == k32 && oi < id);
-            close |= oi != id && !(fabsf(other - k32) > apart);
+            const int2 other = spot[i];
+            const float k = __int_as_float(other.y);
+            rank += k > k32 || (k == k32 && other.x < id);
+            close |= other.x != id && !(fabsf(k - k32) > apart);
         }
-        const float s = rule.softmax ? expf(l - top) * most : 1.f / (1.f + expf(-l));
+        const float s = rule.softmax ? expf(l - top) * most : __fdividef(1.f, 1.f + expf(-l));
         if (!exact && __any_sync(all, live && close)) {  // in 64 bits
-            double s64 = 0., v = -INFINITY;
-            if (live) {
-                s64 = rule.softmax ? exp((double)l - (double)top) / (double)z : sel_sigmoid(l);
-                const float b = bias[id];
-                v = b == b ? s64 + (double)b : -INFINITY;
-            }
-            rank = 0;
-            for (int i = 0; i < n; ++i) {
-                const double ov = __shfl_sync(all, v, i), os = __shfl_sync(all, s64, i);
-                const int oi = __shfl_sync(all, id, i);
-                rank += sel_before(ov, oi, v, id);
-                // (the sum of a softmax has 32 bits: it scales all scores alike)
-                if (rule.softmax && live && os != s64 && fabs(ov - v) <= 2. * err * fabs(os - s64)) sound = false;
-            }
+            const float b = live ? bias[id] : 0.f;
+            rank = sel_rank(row, E, rule.softmax, top, live, l, b, id, n, lane);
         }
         const bool chosen = live && rank < topk;
         float sum = chosen ? s : 0.f;
@@ -380,14 +397,14 @@ __device__ __forceinline__ void select_row(const float *row, const float *bias, 
         if (__all_sync(all, sound)) {
             if (chosen) {
                 picks[rank] = id;
-                weights[rank] = (rule.renorm ? s / sum : s) * rule.scale;
+                weights[rank] = (rule.renorm ? __fdividef(s, sum) : s) * rule.scale;
             }
             if (lane == 0) { picks[topk] = E; weights[topk] = 1.f; }
             return;
         }
     }
     __syncwarp();
-    select_row_slowly(row, bias, E, topk, rule, c, picks, weights, lane);
+    select_row_slowly(row, bias, E, topk, rule, reinterpret_cast<double *>(keys), picks, weights, lane);
 }
 
 }  // namespace gf

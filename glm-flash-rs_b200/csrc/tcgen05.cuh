@@ -118,6 +118,11 @@ __device__ __forceinline__ bool t5_wait(uint64_t *bar, uint32_t parity, volatile
     return false;
 }
 
+// After a give-up: products in flight have read their operands (each takes a fraction of a microsecond).
+__device__ __forceinline__ void t5_settle() {
+    for (int i = 0; i < 100; ++i) __nanosleep(1000);
+}
+
 // position in a ring of barriers and the parity of its phase
 struct T5Ring {
     uint32_t slot = 0, parity = 0;

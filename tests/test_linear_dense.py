@@ -362,3 +362,66 @@ def test_refusals_of_the_binding(pkg, cuda):
                      ((x, w, w), dict(bias_gate=torch.zeros(32, device=cuda), bias_up=torch.zeros(32, device=cuda, dtype=b)))]:
         with pytest.raises(pkg.GlmFlashError):
             pkg.gated_linear(*args, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,K,N", [(300, 4096, 2000), (40, 4096, 1000)])
+def test_status_word(pkg, cuda, rows, K, N):
+    """A status word that is set makes long waits give up; the call returns, the context stays usable, and after a reset results are right."""
+    import torch
+    gen = torch.Generator(device=cuda).manual_seed(7)
+    x, w = torch.randn((rows, K), generator=gen, device=cuda).to(torch.bfloat16), (torch.randn((N, K), generator=gen, device=cuda) / 64).to(torch.bfloat16)
+    want = pkg.linear(x, w)
+    torch.cuda.synchronize()
+    status = pkg.linear_status()
+    assert int(status.item()) == 0
+    status.fill_(3)
+    pkg.linear(x, w)
+    torch.cuda.synchronize()
+    assert int(status.item()) == 3
+    pkg.linear_clear_status()
+    got = pkg.linear(x, w)
+    torch.cuda.synchronize()
+    assert int(status.item()) == 0 and torch.equal(got, want)
+
+
+@pytest.mark.gpu
+def test_the_first_calls_may_be_captured(pkg, cuda):
+    """In a process that has not called anything yet."""
+    import os
+    import subprocess
+    import sys
+    from conftest import ROOT
+    code = f"""
+import sys
+sys.path.insert(0, {ROOT!r})
+import torch
+import __graft_entry__ as entry
+pkg = entry.load_package()
+x = torch.randn(300, 512, device='cuda').to(torch.bfloat16)
+w = torch.randn(256, 512, device='cuda').to(torch.bfloat16)
+bias = torch.randn(256, device='cuda')
+outs = [torch.zeros(r, 256, dtype=torch.bfloat16, device='cuda') for r in (1, 40, 300)]
+gated = torch.zeros(300, 256, dtype=torch.bfloat16, device='cuda')
+logits = torch.zeros(300, 256, device='cuda')
+picks, weights = torch.zeros(300, 5, dtype=torch.int32, device='cuda'), torch.zeros(300, 5, device='cuda')
+def calls():
+    for o in outs:
+        pkg.linear(x[:o.shape[0]], w, out=o)
+    pkg.gated_linear(x, w, w, out=gated)
+    pkg.route_by(x, w, logits, picks, weights, bias=bias)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    calls()
+graph.replay()
+torch.cuda.synchronize()
+kept = [t.clone() for t in outs + [gated, logits, picks, weights]]
+calls()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(kept, outs + [gated, logits, picks, weights]))
+assert float(outs[2].float().abs().sum()) > 0
+print('captured')
+"""
+    env = dict(os.environ)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, env=env, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
