@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(DN_WARPS * 32, MATS * RT == 1 ? 2 : 1) dense_k
 #pragma unroll
         for (int k = 0; k < DN_WARPS; ++k) v[m][0] += part[k][m][r][n];
     }
-    dense_finish<MATS>(a, r, n0 + n, 1, v[0], v[MATS - 1], b);
+    dense_finish<MATS>(a, [&](int) { return r; }, a.rows, n0 + n, v[0], v[MATS - 1], b);
 }
 
 // Which calls of up to 16 rows it takes: those whose CTAs run at once (two an SM for one matrix and up to 8 rows), with few trips a warp.  us, this

@@ -28,8 +28,8 @@ __device__ __forceinline__ float dense_gelu_tanh(float v) { return dense_logisti
 __device__ __forceinline__ float dense_below(float v, float limit) { return v > limit ? limit : v; }
 __device__ __forceinline__ float dense_within(float v, float limit) { return v > limit ? limit : v < -limit ? -limit : v; }
 
-// What follows the sums of output column n of rows r .. r + ROWS - 1, of which the first `count` are there: bias (b), activation and residual, or
-// the gated pair.  Chosen by comparisons around all rows: a jump table in front of every value cost 400 clocks each.
+// What follows the sums of output column n of several rows (row(i), of which those are there that are less than `rows`; row(0) is): bias (b),
+// activation and residual, or the gated pair.  Chosen by comparisons around all rows: a jump table in front of every value cost 400 clocks each.
 template <int ROWS, typename F>
 __device__ __forceinline__ void dense_each(F f) {
 #pragma unroll
@@ -43,14 +43,14 @@ __device__ __forceinline__ void dense_act(float (&v)[ROWS], int act) {
     else if (act == GLMFLASH_ACT_GELU_TANH) dense_each<ROWS>([&](int i) { v[i] = dense_gelu_tanh(v[i]); });
     else dense_each<ROWS>([&](int i) { v[i] = v[i] < 0.f ? 0.f : v[i]; });                                 // (NaN stays)
 }
-template <int MATS, int ROWS>
-__device__ __forceinline__ void dense_finish(const DenseArgs &a, int64_t r, int n, int count, float (&g)[ROWS], float (&u)[ROWS], const float (&b)[2]) {
+template <int MATS, int ROWS, typename R>
+__device__ __forceinline__ void dense_finish(const DenseArgs &a, R row, int rows, int n, float (&g)[ROWS], float (&u)[ROWS], const float (&b)[2]) {
     float res[ROWS];
-    if (MATS == 1 && a.residual) {                       // (rows behind the last one read it once more: no branch between the loads)
-        const int64_t at = r * a.rs + n;
-        if (a.residual_type == GLMFLASH_F32) dense_each<ROWS>([&](int i) { res[i] = static_cast<const float *>(a.residual)[at + min(i, count - 1) * a.rs]; });
-        else if (a.residual_type == GLMFLASH_F16) dense_each<ROWS>([&](int i) { res[i] = __half2float(static_cast<const __half *>(a.residual)[at + min(i, count - 1) * a.rs]); });
-        else dense_each<ROWS>([&](int i) { res[i] = __bfloat162float(static_cast<const __nv_bfloat16 *>(a.residual)[at + min(i, count - 1) * a.rs]); });
+    if (MATS == 1 && a.residual) {                       // (rows that are not there read the first once more: no branch between the loads)
+        auto at = [&](int i) { return (int64_t)(row(i) < rows ? row(i) : row(0)) * a.rs + n; };
+        if (a.residual_type == GLMFLASH_F32) dense_each<ROWS>([&](int i) { res[i] = static_cast<const float *>(a.residual)[at(i)]; });
+        else if (a.residual_type == GLMFLASH_F16) dense_each<ROWS>([&](int i) { res[i] = __half2float(static_cast<const __half *>(a.residual)[at(i)]); });
+        else dense_each<ROWS>([&](int i) { res[i] = __bfloat162float(static_cast<const __nv_bfloat16 *>(a.residual)[at(i)]); });
     }
     dense_each<ROWS>([&](int i) { g[i] += b[0]; });
     if (MATS == 2) {
@@ -60,10 +60,10 @@ __device__ __forceinline__ void dense_finish(const DenseArgs &a, int64_t r, int 
     dense_act(g, a.act);
     if (MATS == 2) dense_each<ROWS>([&](int i) { g[i] *= u[i]; });
     else if (a.residual) dense_each<ROWS>([&](int i) { g[i] += res[i]; });
-    const int64_t at = r * a.os + n;
-    if (a.out_type == GLMFLASH_F32) dense_each<ROWS>([&](int i) { if (i < count) static_cast<float *>(a.out)[at + i * a.os] = g[i]; });
-    else if (a.out_type == GLMFLASH_F16) dense_each<ROWS>([&](int i) { if (i < count) static_cast<__half *>(a.out)[at + i * a.os] = __float2half_rn(g[i]); });
-    else dense_each<ROWS>([&](int i) { if (i < count) static_cast<__nv_bfloat16 *>(a.out)[at + i * a.os] = __float2bfloat16_rn(g[i]); });
+    auto at = [&](int i) { return (int64_t)row(i) * a.os + n; };
+    if (a.out_type == GLMFLASH_F32) dense_each<ROWS>([&](int i) { if (row(i) < rows) static_cast<float *>(a.out)[at(i)] = g[i]; });
+    else if (a.out_type == GLMFLASH_F16) dense_each<ROWS>([&](int i) { if (row(i) < rows) static_cast<__half *>(a.out)[at(i)] = __float2half_rn(g[i]); });
+    else dense_each<ROWS>([&](int i) { if (row(i) < rows) static_cast<__nv_bfloat16 *>(a.out)[at(i)] = __float2bfloat16_rn(g[i]); });
 }
 template <int MATS>
 __device__ __forceinline__ void dense_biases(const DenseArgs &a, int n, float (&b)[2]) {

@@ -30,10 +30,10 @@ constexpr size_t DW_SMEM = 1024 + DW_RING + 256;
 constexpr int DW_REGS_COPY = 40, DW_REGS_EPI = 232;          // launched with 168 x 384: (40 + 2 x 232) x 128
 static_assert(DW_REGS_COPY + 2 * DW_REGS_EPI <= 3 * 168, "registers");
 
-struct DenseMaps { CUtensorMap w[2], x; };
+struct DenseMaps { CUtensorMap a[2], b[2]; };              // M and N operand of the product, or of the two of a gated pair
 
 struct DenseTiles {
-    int bn, across, tiles, stages, pass;                     // rows of a tile, tiles of 256 output columns, all tiles, stages of K, stages of a pass
+    int bn, across, tiles, stages, pass;                     // N of a tile, tiles along M (256), all tiles, stages of K, stages of a pass
     int depth, copies;                                       // stages of the ring, copies that bring a stage of an operand
 };
 
@@ -49,7 +49,7 @@ __device__ __forceinline__ void dense_copy(unsigned char *dst, int stage, int ro
 template <int MATS>
 __device__ __forceinline__ void dense_act32(const DenseArgs &a, float (&v)[32], float b) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] += b;
+    for (int i = 0; i < 32; ++i) v[i] += b;              // (0 where it has been added)
     if (MATS == 2 && a.limit > 0.f) {
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = dense_below(v[i], a.limit);
@@ -78,7 +78,60 @@ __device__ __forceinline__ void dense_store32(const float (&v)[32], void *p, int
     else dense_walk32(static_cast<__nv_bfloat16 *>(p) + at, stride, count, [&](int i, __nv_bfloat16 *q) { if (i < count) __stcs(reinterpret_cast<unsigned short *>(q), __bfloat16_as_ushort(__float2bfloat16_rn(v[i]))); });
 }
 
-template <int MATS, bool CHAIN>
+// The same along a row: 32 neighbouring elements of each lane, 16 bytes at a time where they are aligned and come in that many.
+__device__ __forceinline__ void dense_unpack8(float *v, const uint4 &q, int type) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (type == GLMFLASH_F16) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+            v[2 * i] = f.x; v[2 * i + 1] = f.y;
+        } else {
+            v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+}
+__device__ __forceinline__ void dense_load_along(float (&v)[32], const void *p, int64_t at, int type, int count) {
+    const int size = type == GLMFLASH_F32 ? 4 : 2;
+    const char *q = static_cast<const char *>(p) + at * size;
+    if ((uintptr_t)q % 16 || count * size % 16) return dense_load32(v, p, at, 1, type, count);
+    if (type == GLMFLASH_F32)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) *reinterpret_cast<float4 *>(v + 4 * i) = __ldcs(reinterpret_cast<const float4 *>(q) + min(i, count / 4 - 1));
+    else
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dense_unpack8(v + 8 * i, __ldcs(reinterpret_cast<const uint4 *>(q) + min(i, count / 8 - 1)), type);
+}
+__device__ __forceinline__ void dense_store_along(const float (&v)[32], void *p, int64_t at, int type, int count) {
+    const int size = type == GLMFLASH_F32 ? 4 : 2;
+    char *q = static_cast<char *>(p) + at * size;
+    if ((uintptr_t)q % 16 || count * size % 16) return dense_store32(v, p, at, 1, type, count);
+    if (type == GLMFLASH_F32) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (4 * i < count) __stcs(reinterpret_cast<float4 *>(q) + i, make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]));
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float2 f = make_float2(v[8 * i + 2 * k], v[8 * i + 2 * k + 1]);
+            if (type == GLMFLASH_F16) {
+                const __half2 h = __float22half2_rn(f);
+                w[k] = *reinterpret_cast<const uint32_t *>(&h);
+            } else {
+                const __nv_bfloat162 h = __float22bfloat162_rn(f);
+                w[k] = *reinterpret_cast<const uint32_t *>(&h);
+            }
+        }
+        if (8 * i < count) __stcs(reinterpret_cast<uint4 *>(q) + i, make_uint4(w[0], w[1], w[2], w[3]));
+    }
+}
+
+// ROWS_M: the roles are exchanged, rows of x along M and outputs along N: a lane is a row, a column of tensor memory an output.
+template <int MATS, bool CHAIN, bool ROWS_M>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(DW_THREADS, 1)
 dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, const DenseTiles d) {
     extern __shared__ unsigned char smem_raw[];
@@ -111,20 +164,20 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(DW_REGS_COPY));
         if ((warp == 0 || warp == 3) && lane == 0) {
             const uint32_t full0 = t5_of_cta(full, 0);       // (the copies of both CTAs count on the first one's barrier)
-            const bool rows = warp == 3;
-            const int box = rows ? d.bn >> 1 : 128;
+            const bool along_n = warp == 3;
+            const int box = along_n ? d.bn >> 1 : 128;
             T5Ring at;
             uint32_t it = 0;
             bool ok = true;
             for (int tile = pair; ok && tile < d.tiles; tile += pairs) {
-                const int y = rows ? (tile / d.across) * d.bn + rank * box : (tile % d.across) * 256 + rank * 128;
+                const int y = along_n ? (tile / d.across) * d.bn + rank * box : (tile % d.across) * 256 + rank * 128;
                 for (int m = 0; m < MATS && ok; ++m) {
-                    const CUtensorMap *map = rows ? &maps.x : &maps.w[m];
+                    const CUtensorMap *map = along_n ? &maps.b[m] : &maps.a[m];
                     for (int s = 0; s < d.stages; ++s, ++it) {
                         if (it >= depth && !t5_wait<200>(done + at.slot, at.parity ^ 1, abort_flag, status, GF_STATUS_TMA_TIMEOUT)) { ok = false; break; }
                         if (rank == 0) mbar_expect_tx(full + at.slot, 2 * box * DW_K * 2);
                         const uint32_t bar = full0 + 8 * at.slot;
-                        dense_copy(ring + at.slot * slot_bytes + (rows ? DW_A : 0), s, box, d.copies, [&](unsigned char *to, int k) { t5_load_pair(to, map, d.copies == 1, k, y, bar); });
+                        dense_copy(ring + at.slot * slot_bytes + (along_n ? DW_A : 0), s, box, d.copies, [&](unsigned char *to, int k) { t5_load_pair(to, map, d.copies == 1, k, y, bar); });
                         at.next(depth);
                     }
                 }
@@ -142,14 +195,11 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
             for (int i = 0; i < items * MATS && ok; ++i)
                 for (int s0 = 0; s0 < d.stages && ok; s0 += d.pass, ++pc) {
                     const uint32_t b = pc & 1, acc = tmem + b * DW_ROWS;
-                    ok = __all_sync(0xffffffffu, t5_wait<0>(acc_empty + b, ((pc >> 1) & 1) ^ 1, abort_flag, status, GF_STATUS_MMA_TIMEOUT));
-                    if (!ok) break;
+                    ok = t5_wait<0>(acc_empty + b, ((pc >> 1) & 1) ^ 1, abort_flag, status, GF_STATUS_MMA_TIMEOUT);
                     t5_fence_after();
                     const int end = min(d.pass, d.stages - s0);
                     for (int s = 0; s < end; ++s) {
-                        ok = __all_sync(0xffffffffu, t5_wait<0>(full + at.slot, at.parity, abort_flag, status, GF_STATUS_MMA_TIMEOUT));
-                        if (!ok) break;
-                        t5_fence_after();
+                        ok &= t5_wait<0>(full + at.slot, at.parity, abort_flag, status, GF_STATUS_MMA_TIMEOUT);
                         const uint64_t da = desc0 + at.slot * (slot_bytes >> 4), db = da + (DW_A >> 4);
                         if (t5_elect()) {
 #pragma unroll
@@ -161,6 +211,7 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
                         __syncwarp();
                         at.next(depth);
                     }
+                    ok = __all_sync(0xffffffffu, ok);        // (a vote a stage costs the tensor core 90 clocks of each)
                 }
             if (!ok) t5_settle();
         }
@@ -173,16 +224,22 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
         bool ok = true;
         float keep[4][32];                                   // gated: act(gate) of this lane's rows;  CHAIN: sums
         for (int tile = pair; ok && tile < d.tiles; tile += pairs) {
-            const int n = (tile % d.across) * 256 + rank * 128 + q * 32 + lane, r0 = (tile / d.across) * d.bn + half * cols;
-            const int live = n < a.N ? min(cols, a.rows - r0) : 0;             // rows of this thread
+            // this lane's place along M, the columns' along N, and how many of them there are
+            const int own = (tile % d.across) * 256 + rank * 128 + q * 32 + lane, c0 = (tile / d.across) * d.bn + half * cols;
+            const int live = own < (ROWS_M ? a.rows : a.N) ? min(cols, (ROWS_M ? a.N : a.rows) - c0) : 0;
+            auto place = [&](int c, int64_t stride) { return ROWS_M ? own * stride + c : c * stride + own; };
+            auto load = [&](float (&v)[32], const void *p, int c, int64_t stride, int type, int count) {
+                if (ROWS_M) dense_load_along(v, p, place(c, stride), type, count);
+                else dense_load32(v, p, place(c, stride), stride, type, count);
+            };
 #pragma unroll
             for (int m = 0; m < MATS; ++m) {
-                const float bias = n < a.N && a.bias[m] ? dense_load(a.bias[m], n, a.bias_type) : 0.f;
+                const float bias = !ROWS_M && own < a.N && a.bias[m] ? dense_load(a.bias[m], own, a.bias_type) : 0.f;
                 const int passes = CHAIN ? (d.stages + d.pass - 1) / d.pass : 1;
                 for (int p = 0; p < passes; ++p, ++pc) {
                     const uint32_t b = pc & 1;
                     // (the residual of the first rows is on its way while the pass is multiplied)
-                    if (MATS == 1 && !CHAIN && a.residual && live > 0) dense_load32(keep[0], a.residual, r0 * a.rs + n, a.rs, a.residual_type, live);
+                    if (MATS == 1 && !CHAIN && a.residual && live > 0) load(keep[0], a.residual, c0, a.rs, a.residual_type, min(live, 32));
                     ok = __all_sync(0xffffffffu, t5_wait<200>(acc_full + b, (pc >> 1) & 1, abort_flag, status, GF_STATUS_MMA_TIMEOUT));
                     if (!ok) break;
                     t5_fence_after();
@@ -216,13 +273,18 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
                             __syncwarp();
                             if (lane == 0) t5_arrive_cluster(empty0 + 8 * b);
                         }
-                        const int count = live - 32 * j;
-                        const int64_t row = r0 + 32 * j;
+                        const int count = min(live - 32 * j, 32), c = c0 + 32 * j;
                         if (count > 0) {
+                            if (ROWS_M && a.bias[m]) {
+                                float next[32];
+                                dense_load32(next, a.bias[m], c, 1, a.bias_type, count);
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) v[i] += next[i];
+                            }
                             if (MATS == 1) {
                                 float next[32];
-                                if (a.residual && CHAIN) dense_load32(next, a.residual, row * a.rs + n, a.rs, a.residual_type, count);
-                                if (a.residual && !CHAIN && count > 32) dense_load32(next, a.residual, (row + 32) * a.rs + n, a.rs, a.residual_type, count - 32);
+                                if (a.residual && CHAIN) load(next, a.residual, c, a.rs, a.residual_type, count);
+                                if (a.residual && !CHAIN && live > 32 * j + 32) load(next, a.residual, c + 32, a.rs, a.residual_type, min(live - 32 * j - 32, 32));
                                 dense_act32<1>(a, v, bias);
                                 if (a.residual) {
 #pragma unroll
@@ -236,7 +298,7 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
                             } else {
                                 // (CHAIN: act(gate) waits in its places of the fp32 output)
                                 float gate[32];
-                                if (CHAIN) dense_load32(gate, a.out, row * a.os + n, a.os, GLMFLASH_F32, count);
+                                if (CHAIN) load(gate, a.out, c, a.os, GLMFLASH_F32, count);
 #pragma unroll
                                 for (int i = 0; i < 32; ++i) {
                                     v[i] += bias;
@@ -244,7 +306,10 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
                                     v[i] *= CHAIN ? gate[i] : keep[0][i];
                                 }
                             }
-                            if (MATS == 1 || m == 1 || CHAIN) dense_store32(v, a.out, row * a.os + n, a.os, a.out_type, count);
+                            if (MATS == 1 || m == 1 || CHAIN) {
+                                if (ROWS_M) dense_store_along(v, a.out, place(c, a.os), a.out_type, count);
+                                else dense_store32(v, a.out, place(c, a.os), a.os, a.out_type, count);
+                            }
                         }
                         if (CHAIN || MATS == 2)
 #pragma unroll
@@ -275,7 +340,7 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
 // part, and sends the sums in fours of rows to the CTA of the cluster that finishes them (distributed shared memory, one way, 16 bytes a
 // lane); after a cluster barrier that one adds the parts in ascending order and runs the epilogue.
 //   warps 0, 2 copy weights and rows;  warp 1 allocates tensor memory and issues the products;  warps 4-11 epilogue
-constexpr int DT_THREADS = 384, DT_DEPTH = 8, DT_SMEM = 224 * 1024;
+constexpr int DT_THREADS = 384, DT_DEPTH = 6, DT_SMEM = 224 * 1024;
 
 struct DenseThin {
     int t, row_tiles, stages, chains;                        // rows of a tile (in 16), tiles of rows, stages of K, sums of at most 512 k a CTA
@@ -319,9 +384,9 @@ dense_thin_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
                 mbar_expect_tx(full + at.slot, warp ? d.t * DW_K * 2 : MATS * DW_A);
                 if (warp == 0)
                     for (int m = 0; m < MATS; ++m)
-                        dense_copy(dst + m * DW_A, first + it, 128, d.copies, [&](unsigned char *to, int k) { t5_load(to, &maps.w[m], d.copies == 1, k, n0, full + at.slot); });
+                        dense_copy(dst + m * DW_A, first + it, 128, d.copies, [&](unsigned char *to, int k) { t5_load(to, &maps.a[m], d.copies == 1, k, n0, full + at.slot); });
                 else
-                    dense_copy(dst + MATS * DW_A, first + it, d.t, d.copies, [&](unsigned char *to, int k) { t5_load(to, &maps.x, d.copies == 1, k, r0, full + at.slot); });
+                    dense_copy(dst + MATS * DW_A, first + it, d.t, d.copies, [&](unsigned char *to, int k) { t5_load(to, &maps.b[0], d.copies == 1, k, r0, full + at.slot); });
                 at.next(d.depth);
             }
             // after a give-up: copies in flight have landed before the CTA leaves
@@ -337,35 +402,41 @@ dense_thin_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
         asm volatile("barrier.sync 1, 288;" ::: "memory");   // the epilogue warps may read where it is
         const uint32_t tmem = tmem_slot;
         const uint32_t idesc = t5_idesc(128, d.t, a.type == GLMFLASH_BF16);
-        T5Ring at;
         const uint64_t desc0 = t5_desc(smem_u32(ring));
         const uint32_t next = d.t * 128 >> 4;
         const int chain = (mine + d.chains - 1) / d.chains;
-        int in_chain = 0;
-        uint32_t acc = tmem;
-        for (int it = 0; it < mine && ok; ++it) {
-            ok = __all_sync(0xffffffffu, t5_wait<0>(full + at.slot, at.parity, abort_flag, status, GF_STATUS_MMA_TIMEOUT));
-            if (!ok) break;
-            t5_fence_after();
-            const uint64_t da = desc0 + at.slot * (bytes >> 4), db = da + (MATS * DW_A >> 4);
-            if (in_chain == chain) {                         // the next sum
-                in_chain = 0;
-                acc += d.t;
-            }
-            // (A stage is always multiplied whole, zeros behind K and all: a branch around each product made each take 200 clocks.)
-            if (t5_elect()) {
+        int it = 0, in_chain = 0;
+        uint32_t acc = tmem, parity = 0;
+        // The slots of the ring in line, the lanes' answers collected once a turn of it: with one copy of the code and a vote a stage, 8 products of 96
+        // rows took 690 clocks in place of 525 (the tensor core: 450).
+        while (it < mine && ok) {
 #pragma unroll
-                for (int m = 0; m < MATS; ++m)
+            for (int slot = 0; slot < DT_DEPTH; ++slot) {
+                if (slot < d.depth && it < mine) {
+                    ok &= t5_wait<0>(full + slot, parity, abort_flag, status, GF_STATUS_MMA_TIMEOUT);
+                    const uint64_t da = desc0 + slot * (bytes >> 4), db = da + (MATS * DW_A >> 4);
+                    if (in_chain == chain) {                 // the next sum
+                        in_chain = 0;
+                        acc += d.t;
+                    }
+                    // (A stage is always multiplied whole, zeros behind K and all: a branch around each product made each take 200 clocks.)
+                    if (t5_elect()) {
 #pragma unroll
-                    for (int k = 0; k < DW_K / 16; ++k)
-                        t5_mma<1>(acc + m * d.chains * d.t, da + m * (DW_A >> 4) + 2 * (k & 3) + (k >> 2) * (128 * 128 >> 4), db + 2 * (k & 3) + (k >> 2) * next, idesc,
-                                  k > 0 ? 1u : in_chain > 0);
-                t5_commit<1>(done + at.slot);
-                if (it == mine - 1) t5_commit<1>(&acc_full);
+                        for (int m = 0; m < MATS; ++m)
+#pragma unroll
+                            for (int k = 0; k < DW_K / 16; ++k)
+                                t5_mma<1>(acc + m * d.chains * d.t, da + m * (DW_A >> 4) + 2 * (k & 3) + (k >> 2) * (128 * 128 >> 4), db + 2 * (k & 3) + (k >> 2) * next, idesc,
+                                          k > 0 ? 1u : in_chain > 0);
+                        t5_commit<1>(done + slot);
+                        if (it == mine - 1) t5_commit<1>(&acc_full);
+                    }
+                    __syncwarp();
+                    ++in_chain;
+                    ++it;
+                }
             }
-            __syncwarp();
-            ++in_chain;
-            at.next(d.depth);
+            parity ^= 1;
+            ok = __all_sync(0xffffffffu, ok);
         }
         if (!ok) t5_settle();
     } else if (warp >= 4) {
@@ -403,6 +474,27 @@ dense_thin_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
                     for (int i = 0; i < 32; ++i) v[m][i] += w[i];
                 }
             }
+            if (cn == 1) {                                   // nothing to add
+                const int64_t r = r0 + 32 * j;
+                const int count = n < a.N ? min(32, live - 32 * j) : 0;
+                if (count > 0) {
+                    float res[32];
+                    if (MATS == 1 && a.residual) dense_load32(res, a.residual, r * a.rs + n, a.rs, a.residual_type, count);
+                    dense_act32<MATS>(a, v[0], b[0]);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        if (MATS == 1 && a.residual) v[0][i] += res[i];
+                        if (MATS == 2) {
+                            float u = v[MATS - 1][i] + b[1];
+                            if (a.limit > 0.f) u = dense_within(u, a.limit);
+                            v[0][i] *= u;
+                        }
+                    }
+                    dense_store32(v[0], a.out, r * a.os + n, a.os, a.out_type, count);
+                }
+                __syncwarp();
+                continue;
+            }
             const uint32_t here = smem_u32(parts + rank * d.slots * MATS * 128 + col);
 #pragma unroll
             for (int g = 0; g < 8; ++g) {
@@ -424,24 +516,30 @@ dense_thin_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
     cluster_sync();                                          // the parts of all CTAs have come in
     t5_fence_after();
     if (warp == 1) t5_dealloc<1>(tmem_slot, d.cols);
-    if (warp < 4 || !sound || n >= a.N) return;
+    if (warp < 4 || cn == 1 || !sound || n >= a.N) return;
+    // two fours at a time (the second may be one that is not there: its rows are not live)
 #pragma unroll 1
-    for (int s = half; s * (int)cn + rank < fours; s += 2) {
-        float v[MATS][4];
+    for (int s = half; s * (int)cn + rank < fours; s += 4) {
+        float v[MATS][8];
         const float4 *p = parts + s * MATS * 128 + col;
+        const int second = s + 2 < d.slots ? 2 * MATS * 128 : 0;
 #pragma unroll
-        for (int m = 0; m < MATS; ++m) *reinterpret_cast<float4 *>(v[m]) = p[m * 128];
-#pragma unroll 1
+        for (int m = 0; m < MATS; ++m) {
+            *reinterpret_cast<float4 *>(v[m]) = p[m * 128];
+            *reinterpret_cast<float4 *>(v[m] + 4) = p[second + m * 128];
+        }
+#pragma unroll 2
         for (int c = 1; c < (int)cn; ++c) {
             p += d.slots * MATS * 128;
 #pragma unroll
             for (int m = 0; m < MATS; ++m) {
-                const float4 w = p[m * 128];
+                const float4 w = p[m * 128], y = p[second + m * 128];
                 v[m][0] += w.x; v[m][1] += w.y; v[m][2] += w.z; v[m][3] += w.w;
+                v[m][4] += y.x; v[m][5] += y.y; v[m][6] += y.z; v[m][7] += y.w;
             }
         }
-        const int r = (s * (int)cn + rank) * 4;
-        dense_finish<MATS>(a, r0 + r, n, min(4, live - r), v[0], v[MATS - 1], b);
+        const int r = (s * (int)cn + rank) * 4, r2 = r + 8 * (int)cn;
+        dense_finish<MATS>(a, [&](int i) { return r0 + (i < 4 ? r : r2 - 4) + i; }, r0 + live, n, v[0], v[MATS - 1], b);
     }
 }
 
@@ -461,7 +559,8 @@ static int dense_device(const DenseDevice **out) {
     GF_CUDA(cudaGetDevice(&dev));
     GF_REQUIRE(dev >= 0 && dev < 64, "device ordinal out of range");
     if (!known[dev].sms) {
-        for (auto k : {dense_wide_kernel<1, false>, dense_wide_kernel<1, true>, dense_wide_kernel<2, false>, dense_wide_kernel<2, true>})
+        for (auto k : {dense_wide_kernel<1, false, false>, dense_wide_kernel<1, true, false>, dense_wide_kernel<2, false, false>, dense_wide_kernel<2, true, false>,
+                       dense_wide_kernel<1, false, true>, dense_wide_kernel<1, true, true>, dense_wide_kernel<2, false, true>, dense_wide_kernel<2, true, true>})
             GF_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)DW_SMEM));
         for (auto k : {dense_thin_kernel<1>, dense_thin_kernel<2>}) GF_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, DT_SMEM));
         DenseDevice d = {};
@@ -486,11 +585,15 @@ static int dense_device(const DenseDevice **out) {
     return 0;
 }
 
-static int dense_maps(DenseMaps *maps, const DenseArgs &a, int x_box, int copies) {
+// a and b of the maps: the weights with boxes of 128 and x with boxes of n_box rows, or the roles exchanged
+static int dense_maps(DenseMaps *maps, const DenseArgs &a, bool rows_m, int n_box, int copies) {
     const bool bf = a.type == GLMFLASH_BF16;
-    if (dense_map(&maps->w[0], a.w[0], bf, a.N, a.K, a.ws[0], 128, copies, "weights") || dense_map(&maps->x, a.x, bf, a.rows, a.K, a.xs, x_box, copies, "rows")) return -1;
-    if (a.w[1]) return dense_map(&maps->w[1], a.w[1], bf, a.N, a.K, a.ws[1], 128, copies, "weights");
-    maps->w[1] = maps->w[0];
+    CUtensorMap *w = rows_m ? maps->b : maps->a, *x = rows_m ? maps->a : maps->b;
+    const int w_box = rows_m ? n_box : 128, x_box = rows_m ? 128 : n_box;
+    if (dense_map(&w[0], a.w[0], bf, a.N, a.K, a.ws[0], w_box, copies, "weights") || dense_map(&x[0], a.x, bf, a.rows, a.K, a.xs, x_box, copies, "rows")) return -1;
+    if (a.w[1] && dense_map(&w[1], a.w[1], bf, a.N, a.K, a.ws[1], w_box, copies, "weights")) return -1;
+    if (!a.w[1]) w[1] = w[0];
+    x[1] = x[0];
     return 0;
 }
 
@@ -499,19 +602,22 @@ int dense_gemm(cudaStream_t s, const DenseArgs &a, bool pdl) {
     if (dense_device(&device)) return -1;
     const int pairs = device->sms / 2, mats = a.w[1] ? 2 : 1, stages = (a.K + DW_K - 1) / DW_K, copies = a.K % 64 ? 2 : 1;
     const bool chain = a.out_type == GLMFLASH_F32 && stages > DW_CHAIN;
-    // Wide: rows of a tile, what makes the rounds of tiles over the pairs shortest.  A stage of a round takes 234 ns with 32 rows, 244 with 64, 280
-    // with 128, 312 with 192 (the copies bound it: 42 to 50 bytes a clock and SM) and 386 with 256 (1.61 PFLOP/s: the power limit).
+    // Wide: N of a tile and the operand along M, what makes the rounds of tiles over the pairs shortest.  A stage of a round takes 4 clocks for each of
+    // N on the tensor cores (with 256 on all SMs as long as the power limit says), 0.17 us and more for its copies once all pairs copy.
     DenseTiles d = {};
-    d.across = (a.N + 255) / 256;
+    bool rows_m = false;
     d.stages = stages;
     d.pass = chain ? DW_CHAIN : stages;
     double wide = 1e30;
-    for (int bn = 32; bn <= DW_ROWS; bn += 32) {             // (N of a pair's product goes in 32)
-        const int64_t tiles = (int64_t)((a.rows + bn - 1) / bn) * d.across;
-        const int64_t rounds = (tiles + pairs - 1) / pairs;
-        const double busy = std::min(1., (double)tiles / pairs);
-        const double ns = 5000. + 11. * bn + (double)rounds * stages * mats * std::max({160., 2.05 * bn, busy * (170. + 1.6 * bn)});
-        if (ns <= wide && tiles <= INT32_MAX / 2) { wide = ns; d.bn = bn; d.tiles = (int)tiles; }
+    for (int exchanged = 0; exchanged < 2; ++exchanged) {
+        const int across = ((exchanged ? a.rows : a.N) + 255) / 256, along = exchanged ? a.N : a.rows;
+        for (int bn = 32; bn <= DW_ROWS; bn += 32) {         // (N of a pair's product goes in 32)
+            const int64_t tiles = (int64_t)((along + bn - 1) / bn) * across;
+            const int64_t rounds = (tiles + pairs - 1) / pairs;
+            const double busy = std::min(1., (double)tiles / pairs);
+            const double ns = 5000. + 11. * bn + (double)rounds * stages * mats * std::max({160., 2.05 * bn, busy * (170. + 1.6 * bn)});
+            if ((exchanged ? ns < wide : ns <= wide) && tiles <= INT32_MAX / 2) { wide = ns; rows_m = exchanged; d.bn = bn; d.across = across; d.tiles = (int)tiles; }
+        }
     }
     GF_REQUIRE(wide < 1e30 && (int64_t)(d.tiles / pairs + 1) * mats * stages < INT32_MAX, "the product is too large");
     // Thin: rows of a tile and CTAs that cut K.
@@ -525,7 +631,7 @@ int dense_gemm(cudaStream_t s, const DenseArgs &a, bool pdl) {
         for (int cn = 1; cn <= 8 && cn <= stages; ++cn) {
             if ((int64_t)across * row_tiles > device->clusters[cn]) continue;
             const int most = (stages + cn - 1) / cn, chains = chain ? (most + DW_CHAIN - 1) / DW_CHAIN : 1, bytes = mats * DW_A + t * DW_K * 2;
-            const int slots = (t / 4 + cn - 1) / cn, parts = cn * slots * mats * 2048, need = mats * chains * t + (t % 32 ? 16 : 0);
+            const int slots = (t / 4 + cn - 1) / cn, parts = cn == 1 ? 0 : cn * slots * mats * 2048, need = mats * chains * t + (t % 32 ? 16 : 0);
             if (need > 512 || parts > DT_SMEM - 1024) continue;
             const int room = DT_SMEM - 1024 - parts, apart = std::min(room / bytes, most);
             const bool alias = apart < std::min(3, most);
@@ -543,8 +649,8 @@ int dense_gemm(cudaStream_t s, const DenseArgs &a, bool pdl) {
     }
     DenseMaps maps;
     if (thin < wide) {
-        if (dense_maps(&maps, a, h.t, copies)) return -1;
-        const int bytes = mats * DW_A + h.t * DW_K * 2, parts = cluster * h.slots * mats * 2048;
+        if (dense_maps(&maps, a, false, h.t, copies)) return -1;
+        const int bytes = mats * DW_A + h.t * DW_K * 2, parts = cluster == 1 ? 0 : cluster * h.slots * mats * 2048;
         // At least the share of the shared memory that it takes of the tensor memory: CTAs that fit on an SM side by side (of two streams) then never
         // wait for each other's tensor memory, which CTAs of two clusters could do crosswise, and for good.
         const size_t smem = std::max<size_t>(1024 + (h.alias ? std::max(h.depth * bytes, parts) : h.depth * bytes + parts), (size_t)DT_SMEM * h.cols / 512);
@@ -553,8 +659,11 @@ int dense_gemm(cudaStream_t s, const DenseArgs &a, bool pdl) {
     }
     d.copies = copies;
     d.depth = std::min(DW_RING / (DW_A + d.bn * 128), DW_DEPTH);
-    if (dense_maps(&maps, a, d.bn / 2, copies)) return -1;
-    auto kernel = mats == 2 ? (chain ? dense_wide_kernel<2, true> : dense_wide_kernel<2, false>) : (chain ? dense_wide_kernel<1, true> : dense_wide_kernel<1, false>);
+    if (dense_maps(&maps, a, rows_m, d.bn / 2, copies)) return -1;
+    auto kernel = rows_m ? (mats == 2 ? (chain ? dense_wide_kernel<2, true, true> : dense_wide_kernel<2, false, true>)
+                                      : (chain ? dense_wide_kernel<1, true, true> : dense_wide_kernel<1, false, true>))
+                         : (mats == 2 ? (chain ? dense_wide_kernel<2, true, false> : dense_wide_kernel<2, false, false>)
+                                      : (chain ? dense_wide_kernel<1, true, false> : dense_wide_kernel<1, false, false>));
     return launch_k(kernel, dim3((unsigned)(2 * std::min(d.tiles, pairs))), dim3(DW_THREADS), DW_SMEM, s, pdl, maps, a, d);
 }
 
