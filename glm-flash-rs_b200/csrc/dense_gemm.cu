@@ -340,7 +340,7 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
 // part, and sends the sums in fours of rows to the CTA of the cluster that finishes them (distributed shared memory, one way, 16 bytes a
 // lane); after a cluster barrier that one adds the parts in ascending order and runs the epilogue.
 //   warps 0, 2 copy weights and rows;  warp 1 allocates tensor memory and issues the products;  warps 4-11 epilogue
-constexpr int DT_THREADS = 384, DT_DEPTH = 6, DT_SMEM = 224 * 1024;
+constexpr int DT_THREADS = 384, DT_DEPTH = 8, DT_SMEM = 224 * 1024;
 
 struct DenseThin {
     int t, row_tiles, stages, chains;                        // rows of a tile (in 16), tiles of rows, stages of K, sums of at most 512 k a CTA
@@ -405,39 +405,32 @@ dense_thin_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
         const uint64_t desc0 = t5_desc(smem_u32(ring));
         const uint32_t next = d.t * 128 >> 4;
         const int chain = (mine + d.chains - 1) / d.chains;
-        int it = 0, in_chain = 0;
-        uint32_t acc = tmem, parity = 0;
-        // The slots of the ring in line, the lanes' answers collected once a turn of it: with one copy of the code and a vote a stage, 8 products of 96
-        // rows took 690 clocks in place of 525 (the tensor core: 450).
-        while (it < mine && ok) {
-#pragma unroll
-            for (int slot = 0; slot < DT_DEPTH; ++slot) {
-                if (slot < d.depth && it < mine) {
-                    ok &= t5_wait<0>(full + slot, parity, abort_flag, status, GF_STATUS_MMA_TIMEOUT);
-                    const uint64_t da = desc0 + slot * (bytes >> 4), db = da + (MATS * DW_A >> 4);
-                    if (in_chain == chain) {                 // the next sum
-                        in_chain = 0;
-                        acc += d.t;
-                    }
-                    // (A stage is always multiplied whole, zeros behind K and all: a branch around each product made each take 200 clocks.)
-                    if (t5_elect()) {
-#pragma unroll
-                        for (int m = 0; m < MATS; ++m)
-#pragma unroll
-                            for (int k = 0; k < DW_K / 16; ++k)
-                                t5_mma<1>(acc + m * d.chains * d.t, da + m * (DW_A >> 4) + 2 * (k & 3) + (k >> 2) * (128 * 128 >> 4), db + 2 * (k & 3) + (k >> 2) * next, idesc,
-                                          k > 0 ? 1u : in_chain > 0);
-                        t5_commit<1>(done + slot);
-                        if (it == mine - 1) t5_commit<1>(&acc_full);
-                    }
-                    __syncwarp();
-                    ++in_chain;
-                    ++it;
-                }
+        int in_chain = 0;
+        uint32_t acc = tmem;
+        T5Ring at;
+        for (int it = 0; it < mine; ++it) {
+            ok &= t5_wait<0>(full + at.slot, at.parity, abort_flag, status, GF_STATUS_MMA_TIMEOUT);       // (a vote a stage costs 90 clocks of each)
+            const uint64_t da = desc0 + at.slot * (bytes >> 4), db = da + (MATS * DW_A >> 4);
+            if (in_chain == chain) {                         // the next sum
+                in_chain = 0;
+                acc += d.t;
             }
-            parity ^= 1;
-            ok = __all_sync(0xffffffffu, ok);
+            // (A stage is always multiplied whole, zeros behind K and all: a branch around each product made each take 200 clocks.)
+            if (t5_elect()) {
+#pragma unroll
+                for (int m = 0; m < MATS; ++m)
+#pragma unroll
+                    for (int k = 0; k < DW_K / 16; ++k)
+                        t5_mma<1>(acc + m * d.chains * d.t, da + m * (DW_A >> 4) + 2 * (k & 3) + (k >> 2) * (128 * 128 >> 4), db + 2 * (k & 3) + (k >> 2) * next, idesc,
+                                  k > 0 ? 1u : in_chain > 0);
+                t5_commit<1>(done + at.slot);
+                if (it == mine - 1) t5_commit<1>(&acc_full);
+            }
+            __syncwarp();
+            ++in_chain;
+            at.next(d.depth);
         }
+        ok = __all_sync(0xffffffffu, ok);
         if (!ok) t5_settle();
     } else if (warp >= 4) {
         pdl_wait();
@@ -517,29 +510,23 @@ dense_thin_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
     t5_fence_after();
     if (warp == 1) t5_dealloc<1>(tmem_slot, d.cols);
     if (warp < 4 || cn == 1 || !sound || n >= a.N) return;
-    // two fours at a time (the second may be one that is not there: its rows are not live)
 #pragma unroll 1
-    for (int s = half; s * (int)cn + rank < fours; s += 4) {
-        float v[MATS][8];
+    for (int s = half; s * (int)cn + rank < fours; s += 2) {
+        float v[MATS][4];
         const float4 *p = parts + s * MATS * 128 + col;
-        const int second = s + 2 < d.slots ? 2 * MATS * 128 : 0;
 #pragma unroll
-        for (int m = 0; m < MATS; ++m) {
-            *reinterpret_cast<float4 *>(v[m]) = p[m * 128];
-            *reinterpret_cast<float4 *>(v[m] + 4) = p[second + m * 128];
-        }
-#pragma unroll 2
+        for (int m = 0; m < MATS; ++m) *reinterpret_cast<float4 *>(v[m]) = p[m * 128];
+#pragma unroll 1
         for (int c = 1; c < (int)cn; ++c) {
             p += d.slots * MATS * 128;
 #pragma unroll
             for (int m = 0; m < MATS; ++m) {
-                const float4 w = p[m * 128], y = p[second + m * 128];
+                const float4 w = p[m * 128];
                 v[m][0] += w.x; v[m][1] += w.y; v[m][2] += w.z; v[m][3] += w.w;
-                v[m][4] += y.x; v[m][5] += y.y; v[m][6] += y.z; v[m][7] += y.w;
             }
         }
-        const int r = (s * (int)cn + rank) * 4, r2 = r + 8 * (int)cn;
-        dense_finish<MATS>(a, [&](int i) { return r0 + (i < 4 ? r : r2 - 4) + i; }, r0 + live, n, v[0], v[MATS - 1], b);
+        const int r = (s * (int)cn + rank) * 4;
+        dense_finish<MATS>(a, [&](int i) { return r0 + r + i; }, r0 + live, n, v[0], v[MATS - 1], b);
     }
 }
 
@@ -615,7 +602,7 @@ int dense_gemm(cudaStream_t s, const DenseArgs &a, bool pdl) {
             const int64_t tiles = (int64_t)((along + bn - 1) / bn) * across;
             const int64_t rounds = (tiles + pairs - 1) / pairs;
             const double busy = std::min(1., (double)tiles / pairs);
-            const double ns = 5000. + 11. * bn + (double)rounds * stages * mats * std::max({160., 2.05 * bn, busy * (170. + 1.6 * bn)});
+            const double ns = 5000. + 11. * bn + (double)rounds * mats * (stages * std::max({160., 2.05 * bn, busy * (170. + 1.6 * bn)}) + (chain ? 350. * stages / DW_CHAIN : 0.));
             if ((exchanged ? ns < wide : ns <= wide) && tiles <= INT32_MAX / 2) { wide = ns; rows_m = exchanged; d.bn = bn; d.across = across; d.tiles = (int)tiles; }
         }
     }
