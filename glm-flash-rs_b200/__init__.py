@@ -693,7 +693,7 @@ def _vector(b, N, dt, dev):
 def _matrix(t, rows, cols, dt, dev, what):
     """A residual's or output's type code, address and stride."""
     code = _TYPE_CODES.get(t.dtype, -1)
-    if t.shape != (rows, cols) or t.get_device() != dev:
+    if t.dim() != 2 or t.shape != (rows, cols) or t.get_device() != dev:
         raise GlmFlashError(what + " must be [rows][outer] on x's device")
     if code and t.dtype is not dt:
         raise GlmFlashError(what + " must be float32 or of x's type")
@@ -748,7 +748,12 @@ def _dense(x, w, w_up, out, bias, bias_up, act, residual, out_dtype, limit, stre
                 out = x.new_empty((rows, N), dtype=out_dtype)
     elif out_dtype is not None and out_dtype is not out.dtype:
         raise GlmFlashError("out has another type than out_dtype")
-    ot, op, os_ = _matrix(out, rows, N, dt, dev, "the output")
+    ot = codes.get(out.dtype, -1)
+    os_, side = out.stride() if out.dim() == 2 else (0, 0)
+    if out.shape != (rows, N) or (ot and ot != code) or out.get_device() != dev or (side != 1 and N > 1):
+        _matrix(out, rows, N, dt, dev, "the output")
+    if rows == 1:
+        os_ = N
     if bias is not None:
         bt, bp = _vector(bias, N, dt, dev)
     if bias_up is not None:
@@ -758,7 +763,7 @@ def _dense(x, w, w_up, out, bias, bias_up, act, residual, out_dtype, limit, stre
     if residual is not None:
         rt, rp, rs = _matrix(residual, rows, N, dt, dev, "the residual")
     if call(get_stream(dev) if stream is None else stream.cuda_stream,
-            _LINEAR.pack(x.data_ptr(), w.data_ptr(), up, bp, bu, rp, op, xs, ws, us, rs, os_, rows, K, N, code, bt, rt, ot,
+            _LINEAR.pack(x.data_ptr(), w.data_ptr(), up, bp, bu, rp, out.data_ptr(), xs, ws, us, rs, os_, rows, K, N, code, bt, rt, ot,
                          ACTS[act] if act in ACTS else _named(ACTS, act, "act"), limit, pdl, 0, 0), _LINEAR.size):
         _check(-1)
     return out

@@ -177,7 +177,7 @@ __device__ __noinline__ int sel_rank(const float *row, int E, int softmax, float
 __device__ __forceinline__ void sel_fetch(float *to, const float *from, int E, int lane) {
     const uint32_t at = smem_u32(to);
     if (((uintptr_t)from | E * 4) % 16 == 0)
-        for (int e = 4 * lane; e < E; e += 128) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + 4 * e), "l"(from + e) : "memory");
+        for (int e = 4 * lane; e < E; e += 128) asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(at + 4 * e), "l"(from + e) : "memory");
     else
         for (int e = lane; e < E; e += 32) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(at + 4 * e), "l"(from + e) : "memory");
 }
@@ -374,7 +374,7 @@ __device__ __forceinline__ void select_row(const float *row, const float *bias, 
         const bool live = lane < n;
         const int2 candidate = live ? spot[lane] : make_int2(E, 0);
         const int id = candidate.x;
-        const float k32 = live ? __int_as_float(candidate.y) : -INFINITY, l = live ? clean(row[id]) : 0.f, apart = 2.f * err * (2.f * most + fabsf(k32));
+        const float k32 = live ? __int_as_float(candidate.y) : -INFINITY, l = exact ? k32 : live ? clean(row[id]) : 0.f, apart = 2.f * err * (2.f * most + fabsf(k32));
         int rank = 0;
         bool close = false;
 #pragma unroll 4
