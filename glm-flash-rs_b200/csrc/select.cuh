@@ -188,7 +188,7 @@ __device__ __forceinline__ void sel_fetch(float *to, const float *from, int E, i
 //   2. groups: 32-bit values by a few lanes a group; those that the error could carry over the border are valued in 64 bits by the whole warp
 //   3. a lower bound of the topk-th largest c: of the largest values of the lanes' shares the topk-th; where that leaves more than 32, bisection
 //   4. the candidates, those not provably below it, get a lane each: rank by comparison with all of them, in 64 bits if two are within the error
-// Selection one after another, all in 64 bits (select_row_slowly): 62 us for 8192 rows of 288 experts in 8 groups, 13 us for one row.
+// 8192 rows of 288 experts in 8 groups 13.7 us, one row 3.4; selection one after another, all in 64 bits (select_row_slowly), 62 and 13.
 __device__ __forceinline__ void select_row(const float *row, const float *bias, int E, int topk, const SelRule &rule, float *keys, int2 *spot, int *picks,
                                            float *weights, int lane) {
     const unsigned all = 0xffffffffu;
