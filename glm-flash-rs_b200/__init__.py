@@ -786,7 +786,9 @@ def gated_linear(x, w_gate, w_up, out=None, bias_gate=None, bias_up=None, act="s
 def linear_status():
     """Status word of `linear` and `gated_linear` on the current device: 0, or non-zero when a bounded wait inside a kernel gave up."""
     torch = _torch()
-    return _view(lib().glmflash_linear_status(), (1,), torch.int32)
+    word = lib().glmflash_linear_status()
+    _require(word, "the status word has no address on this device")
+    return _view(word, (1,), torch.int32)
 
 
 def linear_clear_status(stream=None):

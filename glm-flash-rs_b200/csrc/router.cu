@@ -346,6 +346,7 @@ extern "C" int glmflash_topk_by(void *stream, const float *logits, int64_t logit
     if (check_rule(rule, rule_bytes, experts, topk, &sel)) return -1;
     GF_REQUIRE(rows > 0, "rows must be positive");
     GF_REQUIRE(logits_stride >= experts, "logits_stride must be at least the number of experts");
+    GF_REQUIRE(((uintptr_t)logits | (uintptr_t)bias | (uintptr_t)picks | (uintptr_t)weights) % 4 == 0, "logits, bias, picks and weights must be 4-byte aligned");
     return launch_select((cudaStream_t)stream, logits, logits_stride, bias, rows, experts, topk, sel, picks, weights, pdl != 0);
 }
 
@@ -357,6 +358,7 @@ extern "C" int glmflash_route_by(void *stream, const uint16_t *x, int64_t x_stri
     GF_REQUIRE(rows > 0 && hidden > 0 && hidden % 8 == 0, "rows positive; hidden a multiple of 8");
     GF_REQUIRE(x_stride >= hidden && x_stride % 8 == 0, "x_stride must be >= hidden and a multiple of 8");
     GF_REQUIRE(((uintptr_t)x | (uintptr_t)wr) % 16 == 0, "x and the router matrix must be 16-byte aligned");
+    GF_REQUIRE(((uintptr_t)logits | (uintptr_t)bias | (uintptr_t)picks | (uintptr_t)weights) % 4 == 0, "logits, bias, picks and weights must be 4-byte aligned");
     // The dense products, whose kernels are faster than route_kernel for any number of rows and experts (us, logits alone: 2048 x 64 experts, 1 row 2.7
     // | 3.5, 4096 rows 8.3 | 9.5; 4096 x 288, 1 row 3.7 | 18.4, 4096 rows 18.4 | 72.3), and the selection behind them.
     glmflash_linear_args a = {};

@@ -384,7 +384,7 @@ __device__ __forceinline__ void select_row(const float *row, const float *bias, 
             rank += k > k32 || (k == k32 && other.x < id);
             close |= other.x != id && !(fabsf(k - k32) > apart);
         }
-        const float s = rule.softmax ? expf(l - top) * most : __fdividef(1.f, 1.f + expf(-l));
+        const float s = rule.softmax ? expf(l - top) * most : 1.f / (1.f + expf(-l));
         if (!exact && __any_sync(all, live && close)) {  // in 64 bits
             const float b = live ? bias[id] : 0.f;
             rank = sel_rank(row, E, rule.softmax, top, live, l, b, id, n, lane);
@@ -393,7 +393,7 @@ __device__ __forceinline__ void select_row(const float *row, const float *bias, 
         float sum = chosen ? s : 0.f;
 #pragma unroll
         for (int m = 16; m; m >>= 1) sum += __shfl_xor_sync(all, sum, m);
-        if (rule.renorm && sum < 1e-20f) sound = false;  // (scores that 32 bits hold badly, or not at all)
+        if (rule.renorm && __any_sync(all, chosen && s < 1e-30f)) sound = false;       // (scores that 32 bits hold badly, or not at all)
         if (__all_sync(all, sound)) {
             if (chosen) {
                 picks[rank] = id;

@@ -162,6 +162,39 @@ def test_order_of_neighbouring_values(pkg, cuda, scores, group_score):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("scores", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("biased", [False, True])
+def test_small_scores_keep_their_weight(pkg, cuda, scores, biased):
+    """Chosen scores many orders of magnitude apart, down to what 32 bits do not hold: renormalised weights as in 64 bits."""
+    logits = np.full((6, 40), -400.0, np.float32)
+    for r, (a, step) in enumerate([(-30.0, 20.0), (5.0, 40.0), (-87.0, 1.0), (-100.0, 3.0), (-300.0, 5.0), (-60.0, 14.0)]):
+        logits[r, 3:9] = a - step * np.arange(6, dtype=np.float32)
+    bias = np.full(40, -1.0, np.float32)
+    bias[3:9] = [0.5, 0.4, 0.3, 0.2, 0.1, 0.0]                                # (the order of the logits, whatever the scores)
+    b = bias if biased else None
+    want_p, want_w = table(logits, b, 6, scores, scale=2.5)
+    got_p, got_w = run(pkg, cuda, logits, b, 6, scores=scores, scale=2.5)
+    assert np.array_equal(got_p, want_p)
+    assert (np.abs(got_w - want_w) <= WTOL * np.abs(want_w) + 2.5 * 2.0 ** -126).all()
+
+
+@pytest.mark.gpu
+def test_many_ties_and_closed_experts(pkg, cuda):
+    """More candidates than lanes: ties in every row, with and without a bias, experts left open on one lane only, groups with few experts left."""
+    g = np.random.default_rng(3)
+    logits = g.integers(0, 2, (64, 288)).astype(np.float32)
+    closed = np.full(288, -np.inf, np.float32)
+    closed[0::32] = g.standard_normal(9).astype(np.float32) * np.float32(0.1)
+    for b in (None, np.zeros(288, np.float32), np.full(288, 0.125, np.float32), closed):
+        for rule in (dict(), dict(groups=8, keep_groups=1), dict(groups=32, keep_groups=2, group_score="top2"), dict(scores="softmax", groups=4, keep_groups=3, group_score="top2")):
+            r = dict(rule)
+            want_p, _ = table(logits, b, 8, keep=r.pop("keep_groups", None), **r)
+            got_p, got_w = run(pkg, cuda, logits, b, 8, **rule)
+            assert np.array_equal(got_p, want_p), (b is None, rule)
+            assert np.isfinite(got_w).all()
+
+
+@pytest.mark.gpu
 def test_plain_rule_is_topk(pkg, cuda):
     """Sigmoid scores without bias and groups: the table of `topk`."""
     import torch
@@ -245,7 +278,7 @@ def test_refusals(pkg):
                      (dict(groups=0), b"groups"), (dict(groups=33, E=66), b"groups"), (dict(groups=3), b"groups"), (dict(groups=4, keep=5), b"keep_groups"),
                      (dict(groups=4, keep=0), b"keep_groups"), (dict(groups=32, keep=1, k=3), b"topk"), (dict(group_score=2), b"group_score"),
                      (dict(scale=float("nan")), b"scale"), (dict(scale=float("inf")), b"scale"), (dict(res=1), b"reserved"), (dict(size=28), b"size"),
-                     (dict(null=0), b"null"), (dict(null=6), b"null"), (dict(null=8), b"null"), (dict(null=9), b"null")]:
+                     (dict(logits=C.c_void_p(4098)), b"aligned"), (dict(null=0), b"null"), (dict(null=6), b"null"), (dict(null=8), b"null"), (dict(null=9), b"null")]:
         rc, msg = call(**kw)
         assert rc == -1 and word in msg, (kw, msg)
     rule = RULE.pack(0, 1, 1, 0, 1, 1.0, 0, 0)
