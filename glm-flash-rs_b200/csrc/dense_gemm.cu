@@ -15,6 +15,7 @@
 // 8192 x 4096 x 4096 with a residual: 161 us cold at full clocks, the tensor pipe active for 84 % of it; 215 at the power limit.
 // Every wait is bounded; one that gives up sets the status word, every role leaves, copies in flight land, tensor memory is freed.
 #include <algorithm>
+#include <atomic>
 #include <initializer_list>
 
 #include "dense.cuh"
@@ -33,9 +34,19 @@ static_assert(DW_REGS_COPY + 2 * DW_REGS_EPI <= 3 * 168, "registers");
 
 struct DenseMaps { CUtensorMap a[2], b[2]; };              // M and N operand of the product, or of the two of a gated pair
 
+// Tiles in the order of M, a pair's next one without a division.
 struct DenseTiles {
     int bn, across, tiles, stages, pass;                     // N of a tile, tiles along M (256), all tiles, stages of K, stages of a pass
     int depth, copies;                                       // stages of the ring, copies that bring a stage of an operand
+    int step_m, step_n;                                      // from a pair's tile to its next one
+};
+struct DenseTile {
+    int m, n;
+    __device__ __forceinline__ void next(const DenseTiles &d) {
+        m += d.step_m;
+        n += d.step_n;
+        if (m >= d.across) { m -= d.across; ++n; }
+    }
 };
 
 // A stage of `rows` rows: two tiles of 64 k one behind the other.  One copy of a [64][rows][2] box, or two of [64][rows] (K is no multiple of
@@ -58,10 +69,17 @@ __device__ __forceinline__ void dense_act32(const DenseArgs &a, float (&v)[32], 
     dense_act(v, a.act);
 }
 // (Residual and output pass through L2 without pushing operands out: 8192 x 4096 x 4096 with a residual 221 -> 215 us at the power limit.)
-// Walks `count` rows (more than 0) in 32 steps, staying on the last: addresses without a branch between the loads, so that all are on their
-// way at once.
+// f(i, address of row i) for 32 rows, of which `count` (more than 0) are there: the others stand on the last.  Addresses without a branch between the
+// loads, so that all are on their way at once, and each from its own product where the strides allow it (one from another they are a chain of 800
+// clocks for 32 rows).
 template <typename T, typename F>
 __device__ __forceinline__ void dense_walk32(T *p, int64_t stride, int count, F f) {
+    if (stride < 1 << 26) {
+        const int s = (int)stride;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) f(i, p + min(i, count - 1) * s);
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
         f(i, p);
@@ -152,15 +170,17 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
         *abort_flag = 0;
         mbar_fence_init();
     }
+    if (tid < 2 * MATS) asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)(&maps.a[0] + (tid & 1 ? 2 : 0) + (tid >> 1))) : "memory");
     if (warp == 2) t5_alloc<2>(tmem_slot, 512);
+    const int items = (d.tiles - pair + pairs - 1) / pairs;  // (there are no more pairs than tiles)
+    const uint32_t stages = (uint32_t)items * MATS * d.stages, depth = d.depth, slot_bytes = DW_A + d.bn * 128;
+    DenseTile tile = {pair % d.across, pair / d.across};
     t5_fence_before();
     cluster_sync();                                          // the peer's barriers are initialised as well
     t5_fence_after();
     const uint32_t tmem = *tmem_slot;
     pdl_wait();
     pdl_launch_dependents();
-    const int items = d.tiles > pair ? (d.tiles - pair + pairs - 1) / pairs : 0;
-    const uint32_t stages = (uint32_t)items * MATS * d.stages, depth = d.depth, slot_bytes = DW_A + d.bn * 128;
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(DW_REGS_COPY));
         if ((warp == 0 || warp == 3) && lane == 0) {
@@ -170,8 +190,8 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
             T5Ring at;
             uint32_t it = 0;
             bool ok = true;
-            for (int tile = pair; ok && tile < d.tiles; tile += pairs) {
-                const int y = along_n ? (tile / d.across) * d.bn + rank * box : (tile % d.across) * 256 + rank * 128;
+            for (int i = 0; ok && i < items; ++i, tile.next(d)) {
+                const int y = along_n ? tile.n * d.bn + rank * box : tile.m * 256 + rank * 128;
                 for (int m = 0; m < MATS && ok; ++m) {
                     const CUtensorMap *map = along_n ? &maps.b[m] : &maps.a[m];
                     for (int s = 0; s < d.stages; ++s, ++it) {
@@ -221,12 +241,14 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
         const int q = warp & 3, half = (warp - 4) >> 2, cols = d.bn >> 1;
         const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + half * cols;
         const uint32_t empty0 = t5_of_cta(acc_empty, 0);
+        // (nobody waits for the last two passes to be read, and an arrival in the other CTA must not come after that one has left)
+        const uint32_t all = (uint32_t)items * MATS * (CHAIN ? (d.stages + d.pass - 1) / d.pass : 1);
         uint32_t pc = 0;
         bool ok = true;
         float keep[4][32];                                   // gated: act(gate) of this lane's rows;  CHAIN: sums
-        for (int tile = pair; ok && tile < d.tiles; tile += pairs) {
+        for (int i = 0; ok && i < items; ++i, tile.next(d)) {
             // this lane's place along M, the columns' along N, and how many of them there are
-            const int own = (tile % d.across) * 256 + rank * 128 + q * 32 + lane, c0 = (tile / d.across) * d.bn + half * cols;
+            const int own = tile.m * 256 + rank * 128 + q * 32 + lane, c0 = tile.n * d.bn + half * cols;
             const int live = own < (ROWS_M ? a.rows : a.N) ? min(cols, (ROWS_M ? a.N : a.rows) - c0) : 0;
             auto place = [&](int c, int64_t stride) { return ROWS_M ? own * stride + c : c * stride + own; };
             auto load = [&](float (&v)[32], const void *p, int c, int64_t stride, int type, int count) {
@@ -255,7 +277,7 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
                         }
                         t5_fence_before();
                         __syncwarp();
-                        if (lane == 0) t5_arrive_cluster(empty0 + 8 * b);
+                        if (lane == 0 && pc + 2 < all) t5_arrive_cluster(empty0 + 8 * b);
                         if (p < passes - 1) continue;
                     }
                     // One copy of the code that follows the sums: the four groups of 32 rows take turns in keep[0].
@@ -272,7 +294,7 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
                         if (!CHAIN && 32 * (j + 1) >= cols && 32 * j < cols) {  // the last of them: the accumulators are read
                             t5_fence_before();
                             __syncwarp();
-                            if (lane == 0) t5_arrive_cluster(empty0 + 8 * b);
+                            if (lane == 0 && pc + 2 < all) t5_arrive_cluster(empty0 + 8 * b);
                         }
                         const int count = min(live - 32 * j, 32), c = c0 + 32 * j;
                         if (count > 0) {
@@ -326,12 +348,18 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
             }
         }
         // the arrivals of the last commits have come in before this CTA ends
-        for (uint32_t k = stages > depth ? stages - depth : 0; k < stages && ok; ++k)
-            ok = t5_wait<200>(done + k % depth, (k / depth) & 1, abort_flag, status, GF_STATUS_MMA_TIMEOUT);
+        if (warp == 4) {
+            uint32_t slot = stages % depth, parity = stages / depth & 1;               // those of the stage that would come next
+            for (uint32_t k = min(stages, depth); k && ok; --k) {
+                if (slot == 0) { slot = depth; parity ^= 1; }
+                ok = t5_wait<200>(done + --slot, parity, abort_flag, status, GF_STATUS_MMA_TIMEOUT);
+            }
+        }
+        if (!ok) t5_settle();
     }
     t5_fence_before();
-    // the pair ends together (not the aligned form: single lanes of warps 0 and 1 worked alone)
-    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+    // the pair ends together (not the aligned form: single lanes worked alone;  relaxed: what was stored to global memory need not have arrived)
+    asm volatile("barrier.cluster.arrive.relaxed;\n\tbarrier.cluster.wait;" ::: "memory");
     t5_fence_after();
     if (warp == 2) t5_dealloc<2>(tmem, 512);
 }
@@ -341,12 +369,12 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
 // part, and sends the sums in fours of rows to the CTA of the cluster that finishes them (distributed shared memory, one way, 16 bytes a
 // lane); after a cluster barrier that one adds the parts in ascending order and runs the epilogue.
 //   warps 0, 2 copy weights and rows;  warp 1 allocates tensor memory and issues the products;  warps 4-11 epilogue
-// us, calls one behind another: 17 x 2048 x 1536 4.5, 45 x 4096 x 4096 7.4, gated 200 x 4096 x 512 9.3 (63 MB through L2 for 10 MB of operands: K cut six
+// us, calls one behind another: 17 x 2048 x 1536 4.2, 45 x 4096 x 4096 7.2, gated 200 x 4096 x 512 9.2 (63 MB through L2 for 10 MB of operands: K cut six
 // ways, copies of 120 CTAs), 500 x 2048 x 1536 9.2.
 constexpr int DT_THREADS = 384, DT_DEPTH = 8, DT_SMEM = 224 * 1024;
 
 struct DenseThin {
-    int t, row_tiles, stages, chains;                        // rows of a tile (in 16), tiles of rows, stages of K, sums of at most 512 k a CTA
+    int t, share, more, chains;                              // rows of a tile (in 16), stages of a CTA, CTAs that have one more, sums of at most 512 k a CTA
     int depth, copies, slots, alias, cols;                   // stages of the ring, copies that bring a stage of an operand, fours of rows a CTA finishes, the parts lie over the ring, tensor memory
 };
 
@@ -361,10 +389,10 @@ dense_thin_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
     volatile int *abort_flag = &abort_word;
     int *status = &dense_status_word;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    uint32_t cn;
-    asm("mov.u32 %0, %cluster_nctarank;" : "=r"(cn));
-    const int rank = (int)t5_cta_rank(), tile = blockIdx.x / cn, n0 = tile / d.row_tiles * 128, r0 = tile % d.row_tiles * d.t;
-    const int first = (int)((int64_t)d.stages * rank / cn), mine = (int)((int64_t)d.stages * (rank + 1) / cn) - first;    // stages of this CTA
+    // (A cluster is a row of the grid.  Divisions at the start and the end of a call of 5 us cost a tenth of it.)
+    const uint32_t cn = gridDim.x;
+    const int rank = blockIdx.x, n0 = blockIdx.z * 128, r0 = blockIdx.y * d.t;
+    const int first = rank * d.share + min(rank, d.more), mine = d.share + (rank < d.more);              // stages of this CTA
     const uint32_t bytes = MATS * DW_A + (uint32_t)d.t * DW_K * 2;
     float4 *parts = reinterpret_cast<float4 *>(ring + (d.alias ? 0 : (size_t)d.depth * bytes));       // [cn][slots][MATS][128]
     if (tid == 0) {
@@ -407,7 +435,7 @@ dense_thin_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
         const uint32_t idesc = t5_idesc(128, d.t, a.type == GLMFLASH_BF16);
         const uint64_t desc0 = t5_desc(smem_u32(ring));
         const uint32_t next = d.t * 128 >> 4;
-        const int chain = (mine + d.chains - 1) / d.chains;
+        const int chain = d.chains > 1 ? (mine + d.chains - 1) / d.chains : mine;
         int in_chain = 0;
         uint32_t acc = tmem;
         T5Ring at;
@@ -453,7 +481,11 @@ dense_thin_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     if (d.alias) cluster_sync();                             // every CTA has multiplied: the ring is free
     if (warp >= 4 && ok) {
-        const int chain = (mine + d.chains - 1) / d.chains, used = (mine + chain - 1) / chain;      // sums that stages fell to
+        int used = 1;                                        // sums that stages fell to
+        if (d.chains > 1) {
+            const int chain = (mine + d.chains - 1) / d.chains;
+            used = (mine + chain - 1) / chain;
+        }
         const uint32_t lanes = tmem_slot + ((uint32_t)(q * 32) << 16);
 #pragma unroll 1
         for (int j = from; j < to; ++j) {
@@ -545,10 +577,11 @@ static int dense_map(CUtensorMap *map, const void *base, bool bf, int64_t rows, 
 struct DenseDevice { int sms, clusters[9]; };
 static int dense_device(const DenseDevice **out) {
     static DenseDevice known[64] = {};                       // (threads that come here together set the same)
+    static std::atomic<bool> ready[64] = {};
     int dev = 0;
     GF_CUDA(cudaGetDevice(&dev));
     GF_REQUIRE(dev >= 0 && dev < 64, "device ordinal out of range");
-    if (!known[dev].sms) {
+    if (!ready[dev].load(std::memory_order_acquire)) {
         for (auto k : {dense_wide_kernel<1, false, false>, dense_wide_kernel<1, true, false>, dense_wide_kernel<2, false, false>, dense_wide_kernel<2, true, false>,
                        dense_wide_kernel<1, false, true>, dense_wide_kernel<1, true, true>, dense_wide_kernel<2, false, true>, dense_wide_kernel<2, true, true>})
             GF_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)DW_SMEM));
@@ -570,6 +603,7 @@ static int dense_device(const DenseDevice **out) {
         }
         for (int cn = 1; cn <= 8; ++cn) known[dev].clusters[cn] = d.clusters[cn];
         known[dev].sms = d.sms;
+        ready[dev].store(true, std::memory_order_release);
     }
     *out = &known[dev];
     return 0;
@@ -605,14 +639,14 @@ int dense_gemm(cudaStream_t s, const DenseArgs &a, bool pdl) {
             const int64_t tiles = (int64_t)((along + bn - 1) / bn) * across;
             const int64_t rounds = (tiles + pairs - 1) / pairs;
             const double busy = std::min(1., (double)tiles / pairs);
-            const double ns = 5000. + 11. * bn + (double)rounds * mats * (stages * std::max({160., 2.05 * bn, busy * (170. + 1.6 * bn)}) + (chain ? 350. * stages / DW_CHAIN : 0.));
+            const double ns = 4550. + 11. * bn + (double)rounds * mats * (stages * std::max({160., 2.05 * bn, busy * (170. + 1.6 * bn)}) + (chain ? 350. * stages / DW_CHAIN : 0.));
             if ((exchanged ? ns < wide : ns <= wide) && tiles <= INT32_MAX / 2) { wide = ns; rows_m = exchanged; d.bn = bn; d.across = across; d.tiles = (int)tiles; }
         }
     }
     GF_REQUIRE(wide < 1e30 && (int64_t)(d.tiles / pairs + 1) * mats * stages < INT32_MAX, "the product is too large");
     // Thin: rows of a tile and CTAs that cut K.
     DenseThin h = {};
-    int cluster = 0;
+    int cluster = 0, row_split = 0;
     double thin = 1e30;
     const int across = (a.N + 127) / 128;
     for (int tiles = 1; tiles <= 64; ++tiles) {
@@ -628,12 +662,13 @@ int dense_gemm(cudaStream_t s, const DenseArgs &a, bool pdl) {
             const int depth = std::min({alias ? (DT_SMEM - 1024) / bytes : apart, most, DT_DEPTH});
             if (depth < std::min(2, most)) continue;
             const double mma = mats * 8 * std::max({41., 33. + 0.25 * t, 0.5 * t}) / 1.9 + 130.;
-            const double ns = 2440. + most * (154. + 0.54 * std::max({mma, bytes / 150., bytes * (double)(across * row_tiles * cn) / 9000.})) +
+            const double ns = 2090. + most * (154. + 0.54 * std::max({mma, bytes / 150., bytes * (double)(across * row_tiles * cn) / 9000.})) +
                               0.0056 * t * mats * 1024. * (cn - 1) / cn + slots * mats * (88. + 74. * cn);
             if (ns < thin) {
                 thin = ns;
                 cluster = cn;
-                h = {t, row_tiles, stages, chains, depth, copies, slots, alias, need <= 32 ? 32 : need <= 64 ? 64 : need <= 128 ? 128 : need <= 256 ? 256 : 512};
+                row_split = row_tiles;
+                h = {t, stages / cn, stages % cn, chains, depth, copies, slots, alias, need <= 32 ? 32 : need <= 64 ? 64 : need <= 128 ? 128 : need <= 256 ? 256 : 512};
             }
         }
     }
@@ -644,17 +679,20 @@ int dense_gemm(cudaStream_t s, const DenseArgs &a, bool pdl) {
         // At least the share of the shared memory that it takes of the tensor memory: CTAs that fit on an SM side by side (of two streams) then never
         // wait for each other's tensor memory, which CTAs of two clusters could do crosswise, and for good.
         const size_t smem = std::max<size_t>(1024 + (h.alias ? std::max(h.depth * bytes, parts) : h.depth * bytes + parts), (size_t)DT_SMEM * h.cols / 512);
-        return launch_kc(mats == 2 ? dense_thin_kernel<2> : dense_thin_kernel<1>, dim3((unsigned)(across * h.row_tiles * cluster)), dim3(DT_THREADS),
+        return launch_kc(mats == 2 ? dense_thin_kernel<2> : dense_thin_kernel<1>, dim3((unsigned)cluster, (unsigned)row_split, (unsigned)across), dim3(DT_THREADS),
                          dim3((unsigned)cluster), smem, s, pdl, maps, a, h);
     }
     d.copies = copies;
+    const int walking = std::min(d.tiles, pairs);
+    d.step_m = walking % d.across;
+    d.step_n = walking / d.across;
     d.depth = std::min(DW_RING / (DW_A + d.bn * 128), DW_DEPTH);
     if (dense_maps(&maps, a, rows_m, d.bn / 2, copies)) return -1;
     auto kernel = rows_m ? (mats == 2 ? (chain ? dense_wide_kernel<2, true, true> : dense_wide_kernel<2, false, true>)
                                       : (chain ? dense_wide_kernel<1, true, true> : dense_wide_kernel<1, false, true>))
                          : (mats == 2 ? (chain ? dense_wide_kernel<2, true, false> : dense_wide_kernel<2, false, false>)
                                       : (chain ? dense_wide_kernel<1, true, false> : dense_wide_kernel<1, false, false>));
-    return launch_k(kernel, dim3((unsigned)(2 * std::min(d.tiles, pairs))), dim3(DW_THREADS), DW_SMEM, s, pdl, maps, a, d);
+    return launch_k(kernel, dim3((unsigned)(2 * walking)), dim3(DW_THREADS), DW_SMEM, s, pdl, maps, a, d);
 }
 
 }  // namespace gf
