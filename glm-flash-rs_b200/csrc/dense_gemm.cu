@@ -13,6 +13,8 @@
 // first 37 (weights and rows have a thread each): with 64 k and two copies a turn an SM took in 80 GB/s, with one CTA alone as with 148, at any
 // depth of the ring; it can take 117 (all SMs at once).  Where K is a multiple of 64 one copy brings both halves of a stage.
 // 8192 x 4096 x 4096 with a residual: 161 us cold at full clocks, the tensor pipe active for 84 % of it; 215 at the power limit.
+// Loops that wait have no way out of them but their end (one that depends on a wait costs 70 to 120 clocks a turn: 180 to 230 in place of 113), and
+// whole warps run them, of which an elected lane copies or multiplies.
 // Every wait is bounded; one that gives up sets the status word, every role leaves, copies in flight land, tensor memory is freed.
 #include <algorithm>
 #include <atomic>
@@ -183,22 +185,29 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
     pdl_launch_dependents();
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(DW_REGS_COPY));
-        if ((warp == 0 || warp == 3) && lane == 0) {
+        if (warp == 0 || warp == 3) {
             const uint32_t full0 = t5_of_cta(full, 0);       // (the copies of both CTAs count on the first one's barrier)
             const bool along_n = warp == 3;
             const int box = along_n ? d.bn >> 1 : 128;
             T5Ring at;
-            uint32_t it = 0;
+            uint32_t it = 0;                                 // stages that this lane has copied
             bool ok = true;
             for (int i = 0; ok && i < items; ++i, tile.next(d)) {
                 const int y = along_n ? tile.n * d.bn + rank * box : tile.m * 256 + rank * 128;
-                for (int m = 0; m < MATS && ok; ++m) {
+                for (int m = 0; m < MATS; ++m) {
                     const CUtensorMap *map = along_n ? &maps.b[m] : &maps.a[m];
-                    for (int s = 0; s < d.stages; ++s, ++it) {
-                        if (it >= depth && !t5_wait<200>(done + at.slot, at.parity ^ 1, abort_flag, status, GF_STATUS_TMA_TIMEOUT)) { ok = false; break; }
-                        if (rank == 0) mbar_expect_tx(full + at.slot, 2 * box * DW_K * 2);
-                        const uint32_t bar = full0 + 8 * at.slot;
-                        dense_copy(ring + at.slot * slot_bytes + (along_n ? DW_A : 0), s, box, d.copies, [&](unsigned char *to, int k) { t5_load_pair(to, map, d.copies == 1, k, y, bar); });
+#pragma unroll 1
+                    for (int s = 0; s < d.stages; ++s) {
+                        ok &= t5_wait<200>(done + at.slot, at.parity ^ 1, abort_flag, status, GF_STATUS_TMA_TIMEOUT);
+                        if (t5_elect()) {
+                            if (ok) {
+                                if (rank == 0) mbar_expect_tx(full + at.slot, 2 * box * DW_K * 2);
+                                const uint32_t bar = full0 + 8 * at.slot;
+                                dense_copy(ring + at.slot * slot_bytes + (along_n ? DW_A : 0), s, box, d.copies, [&](unsigned char *to, int k) { t5_load_pair(to, map, d.copies == 1, k, y, bar); });
+                                ++it;
+                            }
+                        }
+                        __syncwarp();
                         at.next(depth);
                     }
                 }
@@ -227,11 +236,11 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
                             for (int k = 0; k < DW_K / 16; ++k)
                                 t5_mma<2>(acc, da + 2 * (k & 3) + (k >> 2) * (128 * 128 >> 4), db + 2 * (k & 3) + (k >> 2) * next, idesc, k > 0 ? 1u : s > 0);
                             t5_commit<2>(done + at.slot);
-                            if (s == end - 1) t5_commit<2>(acc_full + b);
                         }
                         __syncwarp();
                         at.next(depth);
                     }
+                    if (t5_elect()) t5_commit<2>(acc_full + b);
                     ok = __all_sync(0xffffffffu, ok);        // (a vote a stage costs the tensor core 90 clocks of each)
                 }
             if (!ok) t5_settle();
@@ -350,9 +359,10 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
         // the arrivals of the last commits have come in before this CTA ends
         if (warp == 4) {
             uint32_t slot = stages % depth, parity = stages / depth & 1;               // those of the stage that would come next
-            for (uint32_t k = min(stages, depth); k && ok; --k) {
+#pragma unroll 1
+            for (uint32_t k = ok ? min(stages, depth) : 0; k; --k) {
                 if (slot == 0) { slot = depth; parity ^= 1; }
-                ok = t5_wait<200>(done + --slot, parity, abort_flag, status, GF_STATUS_MMA_TIMEOUT);
+                ok &= t5_wait<200>(done + --slot, parity, abort_flag, status, GF_STATUS_MMA_TIMEOUT);
             }
         }
         if (!ok) t5_settle();
@@ -388,7 +398,7 @@ dense_thin_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
     __shared__ int abort_word;
     volatile int *abort_flag = &abort_word;
     int *status = &dense_status_word;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = tid >> 5;
     // (A cluster is a row of the grid.  Divisions at the start and the end of a call of 5 us cost a tenth of it.)
     const uint32_t cn = gridDim.x;
     const int rank = blockIdx.x, n0 = blockIdx.z * 128, r0 = blockIdx.y * d.t;
@@ -406,24 +416,29 @@ dense_thin_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
     bool ok = true;
     if (warp == 0 || warp == 2) {                            // (they do not wait for the tensor memory)
         pdl_wait();
-        if (lane == 0) {
-            T5Ring at;
-            int it = 0;
-            for (; it < mine; ++it) {
-                if (it >= d.depth && !t5_wait<200>(done + at.slot, at.parity ^ 1, abort_flag, status, GF_STATUS_TMA_TIMEOUT)) break;
-                unsigned char *dst = ring + (size_t)at.slot * bytes;
-                mbar_expect_tx(full + at.slot, warp ? d.t * DW_K * 2 : MATS * DW_A);
-                if (warp == 0)
-                    for (int m = 0; m < MATS; ++m)
-                        dense_copy(dst + m * DW_A, first + it, 128, d.copies, [&](unsigned char *to, int k) { t5_load(to, &maps.a[m], d.copies == 1, k, n0, full + at.slot); });
-                else
-                    dense_copy(dst + MATS * DW_A, first + it, d.t, d.copies, [&](unsigned char *to, int k) { t5_load(to, &maps.b[0], d.copies == 1, k, r0, full + at.slot); });
-                at.next(d.depth);
+        T5Ring at;
+        int copied = 0;                                      // stages that this lane has copied
+#pragma unroll 1
+        for (int it = 0; it < mine; ++it) {
+            ok &= t5_wait<200>(done + at.slot, at.parity ^ 1, abort_flag, status, GF_STATUS_TMA_TIMEOUT);
+            if (t5_elect()) {
+                if (ok) {
+                    unsigned char *dst = ring + (size_t)at.slot * bytes;
+                    mbar_expect_tx(full + at.slot, warp ? d.t * DW_K * 2 : MATS * DW_A);
+                    if (warp == 0)
+                        for (int m = 0; m < MATS; ++m)
+                            dense_copy(dst + m * DW_A, first + it, 128, d.copies, [&](unsigned char *to, int k) { t5_load(to, &maps.a[m], d.copies == 1, k, n0, full + at.slot); });
+                    else
+                        dense_copy(dst + MATS * DW_A, first + it, d.t, d.copies, [&](unsigned char *to, int k) { t5_load(to, &maps.b[0], d.copies == 1, k, r0, full + at.slot); });
+                    ++copied;
+                }
             }
-            // after a give-up: copies in flight have landed before the CTA leaves
-            if (it < mine || *abort_flag)
-                for (int k = max(it - d.depth, 0); k < it; ++k) mbar_wait(full + k % d.depth, (k / d.depth) & 1, nullptr, 1000u);
+            __syncwarp();
+            at.next(d.depth);
         }
+        // after a give-up: copies in flight have landed before the CTA leaves
+        if (!ok || *abort_flag)
+            for (int k = max(copied - d.depth, 0); k < copied; ++k) mbar_wait(full + k % d.depth, (k / d.depth) & 1, nullptr, 1000u);
     } else if (warp == 1) {
         // (The next kernel of the stream may start only now: one that took the SM's tensor memory first would wait for this one, which waits for it.)
         t5_alloc<1>(&tmem_slot, d.cols);
@@ -455,12 +470,12 @@ dense_thin_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
                         t5_mma<1>(acc + m * d.chains * d.t, da + m * (DW_A >> 4) + 2 * (k & 3) + (k >> 2) * (128 * 128 >> 4), db + 2 * (k & 3) + (k >> 2) * next, idesc,
                                   k > 0 ? 1u : in_chain > 0);
                 t5_commit<1>(done + at.slot);
-                if (it == mine - 1) t5_commit<1>(&acc_full);
             }
             __syncwarp();
             ++in_chain;
             at.next(d.depth);
         }
+        if (t5_elect()) t5_commit<1>(&acc_full);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) t5_settle();
     } else if (warp >= 4) {
