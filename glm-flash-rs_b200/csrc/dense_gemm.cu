@@ -252,6 +252,8 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
         const uint32_t empty0 = t5_of_cta(acc_empty, 0);
         // (nobody waits for the last two passes to be read, and an arrival in the other CTA must not come after that one has left)
         const uint32_t all = (uint32_t)items * MATS * (CHAIN ? (d.stages + d.pass - 1) / d.pass : 1);
+        constexpr bool EARLY = MATS == 1 && !CHAIN;
+        const int turns = CHAIN || MATS == 2 ? 4 : (cols + 31) >> 5;
         uint32_t pc = 0;
         bool ok = true;
         float keep[4][32];                                   // gated: act(gate) of this lane's rows;  CHAIN: sums
@@ -271,10 +273,12 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
                 for (int p = 0; p < passes; ++p, ++pc) {
                     const uint32_t b = pc & 1;
                     // (the residual of the first rows is on its way while the pass is multiplied)
-                    if (MATS == 1 && !CHAIN && a.residual && live > 0) load(keep[0], a.residual, c0, a.rs, a.residual_type, min(live, 32));
-                    ok = __all_sync(0xffffffffu, t5_wait<200>(acc_full + b, (pc >> 1) & 1, abort_flag, status, GF_STATUS_MMA_TIMEOUT));
-                    if (!ok) break;
-                    t5_fence_after();
+                    if (MATS == 1 && !CHAIN && a.residual && live > 0 && (!EARLY || i)) load(keep[0], a.residual, c0, a.rs, a.residual_type, min(live, 32));
+                    if (!EARLY) {
+                        ok = __all_sync(0xffffffffu, t5_wait<200>(acc_full + b, (pc >> 1) & 1, abort_flag, status, GF_STATUS_MMA_TIMEOUT));
+                        if (!ok) break;
+                        t5_fence_after();
+                    }
                     if (CHAIN) {
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
@@ -289,23 +293,33 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
                         if (lane == 0 && pc + 2 < all) t5_arrive_cluster(empty0 + 8 * b);
                         if (p < passes - 1) continue;
                     }
-                    // One copy of the code that follows the sums: the four groups of 32 rows take turns in keep[0].
+                    // One copy of the code that follows the sums: the four groups of 32 rows take turns in keep[0].  A pair's first tile has a turn more,
+                    // of no rows, while it is multiplied: it brings the instructions in, which took longer than they do, and the first residual
+                    // (1000 x 2048 x 1536 10.4 -> 10.1 us; registers do not last for it in a gated pair).
 #pragma unroll 1
-                    for (int j = 0; j < 4; ++j) {
+                    for (int j = EARLY && !i ? -1 : 0; j < turns; ++j) {
                         float v[32];
+                        if (EARLY && j == 0) {
+                            ok = __all_sync(0xffffffffu, t5_wait<200>(acc_full + b, (pc >> 1) & 1, abort_flag, status, GF_STATUS_MMA_TIMEOUT));
+                            if (!ok) break;
+                            t5_fence_after();
+                        }
                         __syncwarp();
                         if (CHAIN) {
 #pragma unroll
                             for (int i = 0; i < 32; ++i) v[i] = keep[0][i];
-                        } else if (32 * j < cols) {
+                        } else if ((!EARLY || j >= 0) && 32 * j < cols) {
                             t5_ld32(lanes + b * DW_ROWS + 32 * j, v);
+                        } else if (EARLY) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) v[i] = 0.f;
                         }
-                        if (!CHAIN && 32 * (j + 1) >= cols && 32 * j < cols) {  // the last of them: the accumulators are read
+                        if (!CHAIN && (!EARLY || j >= 0) && 32 * (j + 1) >= cols && 32 * j < cols) {  // the last of them: the accumulators are read
                             t5_fence_before();
                             __syncwarp();
                             if (lane == 0 && pc + 2 < all) t5_arrive_cluster(empty0 + 8 * b);
                         }
-                        const int count = min(live - 32 * j, 32), c = c0 + 32 * j;
+                        const int here = EARLY ? 32 * max(j, 0) : 32 * j, ahead = 32 * (j + 1), count = min(live - here, 32), c = c0 + here;
                         if (count > 0) {
                             if (ROWS_M && a.bias[m]) {
                                 float next[32];
@@ -316,7 +330,7 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
                             if (MATS == 1) {
                                 float next[32];
                                 if (a.residual && CHAIN) load(next, a.residual, c, a.rs, a.residual_type, count);
-                                if (a.residual && !CHAIN && live > 32 * j + 32) load(next, a.residual, c + 32, a.rs, a.residual_type, min(live - 32 * j - 32, 32));
+                                if (a.residual && !CHAIN && live > ahead) load(next, a.residual, c0 + ahead, a.rs, a.residual_type, min(live - ahead, 32));
                                 dense_act32<1>(a, v, bias);
                                 if (a.residual) {
 #pragma unroll
@@ -339,8 +353,9 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
                                 }
                             }
                             if (MATS == 1 || m == 1 || CHAIN) {
-                                if (ROWS_M) dense_store_along(v, a.out, place(c, a.os), a.out_type, count);
-                                else dense_store32(v, a.out, place(c, a.os), a.os, a.out_type, count);
+                                const int stored = EARLY && j < 0 ? 0 : count;
+                                if (ROWS_M) dense_store_along(v, a.out, place(c, a.os), a.out_type, stored);
+                                else dense_store32(v, a.out, place(c, a.os), a.os, a.out_type, stored);
                             }
                         }
                         if (CHAIN || MATS == 2)
