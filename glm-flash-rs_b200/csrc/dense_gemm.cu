@@ -166,8 +166,12 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
     int *status = &dense_status_word;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = (int)t5_cta_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    if (tid < DW_DEPTH) {
+        mbar_init(full + tid, 2);
+        mbar_init(done + tid, 1);
+        mbar_fence_init();
+    }
     if (tid == 0) {
-        for (int s = 0; s < DW_DEPTH; ++s) { mbar_init(full + s, 2); mbar_init(done + s, 1); }
         for (int b = 0; b < 2; ++b) { mbar_init(acc_full + b, 1); mbar_init(acc_empty + b, 16); }
         *abort_flag = 0;
         mbar_fence_init();
@@ -420,12 +424,17 @@ dense_thin_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
     const int first = rank * d.share + min(rank, d.more), mine = d.share + (rank < d.more);              // stages of this CTA
     const uint32_t bytes = MATS * DW_A + (uint32_t)d.t * DW_K * 2;
     float4 *parts = reinterpret_cast<float4 *>(ring + (d.alias ? 0 : (size_t)d.depth * bytes));       // [cn][slots][MATS][128]
-    if (tid == 0) {
-        for (int s = 0; s < d.depth; ++s) { mbar_init(full + s, 2); mbar_init(done + s, 1); }
-        mbar_init(&acc_full, 1);
-        abort_word = 0;
+    if (tid < DT_DEPTH) {
+        mbar_init(full + tid, 2);
+        mbar_init(done + tid, 1);
+        if (tid == 0) {
+            mbar_init(&acc_full, 1);
+            abort_word = 0;
+        }
         mbar_fence_init();
     }
+    // (by a warp that has nothing else to do: 2048 x 512 4.95 us instead of 5.12)
+    if (tid >= 96 && tid <= 96 + MATS) asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)(tid == 96 ? &maps.b[0] : &maps.a[tid - 97])) : "memory");
     __syncthreads();
     asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");     // (waited for in front of the first store to a peer)
     bool ok = true;
