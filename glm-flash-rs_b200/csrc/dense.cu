@@ -2,6 +2,7 @@
 // out = act(min(x . wg^T + bg, limit)) * clamp(x . wu^T + bu, -limit, limit), fp16 or bf16 operands, fp32 sums, one rounding at the end.
 // The projections around the expert path that a checkpoint keeps dense (the shared expert of an upstream bank, a vocabulary head).
 #include "dense.cuh"
+#include "select.cuh"
 
 namespace gf {
 
@@ -34,11 +35,10 @@ __device__ __forceinline__ uint4 dense_ldg(const void *p) {
 // one.  The k slots of a fragment may be any as long as both operands agree: a lane loads 16 contiguous bytes of a row (k = 8 t .. 8 t + 7 of a step) and
 // uses them as the fragments of two instructions.
 constexpr int DN_N = 16, DN_WARPS = 16, DN_AHEAD = 4;
-template <bool BF, int MATS, int RT>
-__global__ void __launch_bounds__(DN_WARPS * 32, MATS * RT == 1 ? 2 : 1) dense_kernel(const DenseArgs a) {
-    __shared__ float part[DN_WARPS][MATS][8 * RT][DN_N + 1];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int n0 = blockIdx.x * DN_N, whole = a.K >> 5;
+// start() once the kernel in front has ended, finish(row, column, sums) for what this thread has of them.
+template <bool BF, int MATS, int RT, typename S, typename F>
+__device__ __forceinline__ void dense_columns(const DenseArgs &a, int n0, S start, F finish, float (&part)[DN_WARPS][MATS][8 * RT][DN_N + 1]) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3, whole = a.K >> 5;
     const uint16_t *w[MATS][2];
 #pragma unroll
     for (int m = 0; m < MATS; ++m)
@@ -54,6 +54,7 @@ __global__ void __launch_bounds__(DN_WARPS * 32, MATS * RT == 1 ? 2 : 1) dense_k
             }
     pdl_wait();
     pdl_launch_dependents();
+    start();
     const uint16_t *x = static_cast<const uint16_t *>(a.x) + g * a.xs + 8 * t;
     float acc[MATS][RT][4] = {};
     const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
@@ -106,15 +107,55 @@ __global__ void __launch_bounds__(DN_WARPS * 32, MATS * RT == 1 ? 2 : 1) dense_k
     __syncthreads();
     const int r = tid / DN_N, n = tid % DN_N;
     if (tid >= 8 * RT * DN_N || r >= a.rows || n0 + n >= a.N) return;
-    float v[MATS][1], b[2];
-    dense_biases<MATS>(a, n0 + n, b);
+    float v[MATS][1];
 #pragma unroll
     for (int m = 0; m < MATS; ++m) {
         v[m][0] = 0.f;
 #pragma unroll
         for (int k = 0; k < DN_WARPS; ++k) v[m][0] += part[k][m][r][n];
     }
-    dense_finish<MATS>(a, [&](int) { return r; }, a.rows, n0 + n, v[0], v[MATS - 1], b);
+    finish(r, n0 + n, v);
+}
+template <bool BF, int MATS, int RT>
+__global__ void __launch_bounds__(DN_WARPS * 32, MATS * RT == 1 ? 2 : 1) dense_kernel(const DenseArgs a) {
+    __shared__ float part[DN_WARPS][MATS][8 * RT][DN_N + 1];
+    dense_columns<BF, MATS, RT>(a, blockIdx.x * DN_N, [] {}, [&](int r, int n, float (&v)[MATS][1]) {
+        float b[2];
+        dense_biases<MATS>(a, n, b);
+        dense_finish<MATS>(a, [&](int) { return r; }, a.rows, n, v[0], v[MATS - 1], b);
+    }, part);
+}
+
+// The router of up to 16 rows in one launch: a cluster of up to eight CTAs has the columns between them and sends each logit to the shared memory of the
+// CTA whose warp selects that row.  Two launches wait for the first one's stores and end, and cost the host
+// 2 us more.  us in a graph, 2048 x 64, 1, 8 and 16 rows: 4.3, 4.7, 5.3 instead of 5.0, 5.4, 6.0; 4096 x 128, 1 row: 5.2 instead of 6.2.  With two blocks of
+// columns a CTA (2048 x 256, 1 row) the one launch takes 7.6, two 5.4.
+template <int RT>
+__global__ void __launch_bounds__(DN_WARPS * 32, 1) dense_route_kernel(const DenseArgs a, const float *bias, int topk, SelRule rule, int *picks, float *weights) {
+    extern __shared__ double route_values[];                 // of each of this CTA's rows: keys, biases, logits
+    __shared__ float part[DN_WARPS][1][8 * RT][DN_N + 1];
+    __shared__ int2 spot[DN_WARPS][32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cn = gridDim.x, r = blockIdx.x + warp * cn, wide = (a.N + 31) / 32 * 32;
+    float *keys = reinterpret_cast<float *>(route_values) + warp * 3 * wide;
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");     // (waited for in front of the first store to a peer)
+    int row = -1, column = 0;
+    float logit = 0.f;
+    auto fetch = [&] {
+        if (r >= a.rows) return;
+        if (bias) sel_fetch(keys + wide, bias, a.N, lane);
+        sel_pad(keys, a.N, bias != nullptr, lane);
+    };
+    dense_columns<true, 1, RT>(a, blockIdx.x * DN_N, fetch, [&](int r, int n, float (&v)[1][1]) { row = r; column = n; logit = v[0][0]; }, part);
+    __syncwarp();
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (row >= 0) {
+        float *to = const_cast<float *>(cluster_map(reinterpret_cast<float *>(route_values) + row / cn * 3 * wide + column, row % cn));
+        to[0] = to[2 * wide] = logit;
+    }
+    __syncwarp();
+    cluster_sync();
+    if (row >= 0) static_cast<float *>(a.out)[row * a.os + column] = logit;
+    if (r < a.rows) select_row<true>(keys + 2 * wide, bias, a.N, topk, rule, keys, spot[warp], picks + r * (topk + 1), weights + r * (topk + 1), lane);
 }
 
 // Which calls of up to 16 rows it takes: those whose CTAs run at once (two an SM for one matrix and up to 8 rows), with few trips a warp.  us, this
@@ -132,6 +173,14 @@ template <bool BF, int MATS>
 static int launch_dense(cudaStream_t s, const DenseArgs &a, bool pdl) {
     const dim3 grid((unsigned)((a.N + DN_N - 1) / DN_N)), block(DN_WARPS * 32);
     return a.rows > 8 ? launch_k(dense_kernel<BF, MATS, 2>, grid, block, 0, s, pdl, a) : launch_k(dense_kernel<BF, MATS, 1>, grid, block, 0, s, pdl, a);
+}
+
+bool dense_route_fits(const DenseArgs &a) { return dense_small(a) && a.N <= 8 * DN_N; }
+int dense_route(cudaStream_t s, const DenseArgs &a, const float *bias, int topk, const SelRule &rule, int *picks, float *weights, bool pdl) {
+    const int cn = std::min((a.N + DN_N - 1) / DN_N, 8);
+    const size_t smem = (size_t)((a.rows + cn - 1) / cn) * ((a.N + 31) / 32 * 32) * 3 * sizeof(float);
+    return launch_kc(a.rows > 8 ? dense_route_kernel<2> : dense_route_kernel<1>, dim3((unsigned)cn), dim3(DN_WARPS * 32), dim3((unsigned)cn), smem, s, pdl, a, bias, topk, rule,
+                     picks, weights);
 }
 
 }  // namespace gf

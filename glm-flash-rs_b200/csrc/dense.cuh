@@ -72,5 +72,9 @@ __device__ __forceinline__ void dense_biases(const DenseArgs &a, int n, float (&
 }
 
 int dense_gemm(cudaStream_t s, const DenseArgs &a, bool pdl);
+// Router product (bf16, fp32 output) and selection in one launch, where they fit a cluster
+struct SelRule;
+bool dense_route_fits(const DenseArgs &a);
+int dense_route(cudaStream_t s, const DenseArgs &a, const float *bias, int topk, const SelRule &rule, int *picks, float *weights, bool pdl);
 
 }  // namespace gf

@@ -5,6 +5,7 @@
 //   weight = score / sum of the chosen scores; the row's last slot is the shared expert (id E) with weight 1.
 // Selection is done on the logits (sigmoid is monotonic), so it does not depend on the precision of expf.
 #include "common.cuh"
+#include "dense.cuh"
 #include "select.cuh"
 
 namespace gf {
@@ -255,7 +256,7 @@ __global__ void __launch_bounds__(SEL_WARPS * 32, 8) select_kernel(const float *
     pdl_wait();
     pdl_launch_dependents();
     if (r >= rows) return;
-    select_row(logits + r * stride, bias, E, topk, rule, reinterpret_cast<float *>(sel_values) + warp * ((E + 31) / 32 * (bias ? 64 : 32)), spot[warp],
+    select_row<false>(logits + r * stride, bias, E, topk, rule, reinterpret_cast<float *>(sel_values) + warp * ((E + 31) / 32 * (bias ? 64 : 32)), spot[warp],
                picks + r * (topk + 1), weights + r * (topk + 1), lane);
 }
 
@@ -360,7 +361,13 @@ extern "C" int glmflash_route_by(void *stream, const uint16_t *x, int64_t x_stri
     GF_REQUIRE(((uintptr_t)x | (uintptr_t)wr) % 16 == 0, "x and the router matrix must be 16-byte aligned");
     GF_REQUIRE(((uintptr_t)logits | (uintptr_t)bias | (uintptr_t)picks | (uintptr_t)weights) % 4 == 0, "logits, bias, picks and weights must be 4-byte aligned");
     // The dense products, whose kernels are faster than route_kernel for any number of rows and experts (us, logits alone: 2048 x 64 experts, 1 row 2.7
-    // | 3.5, 4096 rows 8.3 | 9.5; 4096 x 288, 1 row 3.7 | 18.4, 4096 rows 18.4 | 72.3), and the selection behind them.
+    // | 3.5, 4096 rows 8.3 | 9.5; 4096 x 288, 1 row 3.7 | 18.4, 4096 rows 18.4 | 72.3), and the selection behind them: in the same
+    // launch for few rows and experts.
+    if (rows <= 16) {
+        const DenseArgs few = {x, {wr, nullptr}, {nullptr, nullptr}, nullptr, logits, x_stride, {hidden, 0}, 0, experts, rows, hidden, experts, GLMFLASH_BF16, GLMFLASH_F32, GLMFLASH_F32,
+                               GLMFLASH_F32, GLMFLASH_ACT_NONE, 0.f};
+        if (dense_route_fits(few)) return dense_route((cudaStream_t)stream, few, bias, topk, sel, picks, weights, pdl != 0);
+    }
     glmflash_linear_args a = {};
     a.x = x;
     a.w = wr;

@@ -28,7 +28,7 @@ __device__ __forceinline__ bool sel_before(double a, int i, double b, int j) { r
 __device__ __forceinline__ double sel_sigmoid(double l) { return 1. / (1. + exp(-l)); }
 
 // One row by one warp in 64 bits throughout: whatever select_row leaves undecided.  c: E doubles of shared memory of this warp's (with a bias).
-__device__ __noinline__ void select_row_slowly(const float *row, const float *bias, int E, int topk, const SelRule &rule, double *c, int *picks,
+static __device__ __noinline__ void select_row_slowly(const float *row, const float *bias, int E, int topk, const SelRule &rule, double *c, int *picks,
                                                float *weights, int lane) {
     const unsigned all = 0xffffffffu;
     double top = 0., z = 1.;                             // softmax: the largest logit, the sum
@@ -126,7 +126,7 @@ __device__ __forceinline__ double sel_sum(const float *row, int E, float top, in
     return sum;
 }
 // of the groups in `left` (the bits of their lanes, `wide` a group) how many come before this lane's, by their values in 64 bits
-__device__ __noinline__ int sel_groups_before(const float *row, const float *bias, int E, const SelRule &rule, float top, unsigned left, int wide, int lane) {
+static __device__ __noinline__ int sel_groups_before(const float *row, const float *bias, int E, const SelRule &rule, float top, unsigned left, int wide, int lane) {
     const unsigned all = 0xffffffffu;
     const int per = E / rule.groups, g = lane / wide;
     // (without a bias a softmax's sum is left out: it scales all alike)
@@ -163,7 +163,7 @@ __device__ __noinline__ int sel_groups_before(const float *row, const float *bia
     return before;
 }
 // rank of this lane's candidate (logit l, bias b) among n by c in 64 bits
-__device__ __noinline__ int sel_rank(const float *row, int E, int softmax, float top, bool live, float l, float b, int id, int n, int lane) {
+static __device__ __noinline__ int sel_rank(const float *row, int E, int softmax, float top, bool live, float l, float b, int id, int n, int lane) {
     const double sum64 = softmax ? sel_sum(row, E, top, lane) : 1.;
     double v = -INFINITY;
     if (live && b == b) v = (softmax ? exp((double)l - (double)top) / sum64 : sel_sigmoid(l)) + (double)b;
@@ -182,6 +182,15 @@ __device__ __forceinline__ void sel_fetch(float *to, const float *from, int E, i
         for (int e = lane; e < E; e += 32) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(at + 4 * e), "l"(from + e) : "memory");
 }
 
+// behind the last expert
+__device__ __forceinline__ void sel_pad(float *keys, int E, bool biased, int lane) {
+    const int turns = (E + 31) >> 5, e = lane + 32 * (turns - 1);
+    if (e >= E) {
+        keys[e] = -INFINITY;
+        if (biased) keys[32 * turns + e] = -INFINITY;
+    }
+}
+
 // One row by one warp; E <= 1024, topk <= 31, groups <= 32.  keys: shared memory of this warp's, a multiple of 32 experts floats, as many again behind
 // them with a bias; spot: 32 places.
 //   1. 32-bit c of every expert, in shared memory (in registers the loops over them have to be unrolled: long code, fetched for one pass)
@@ -189,6 +198,8 @@ __device__ __forceinline__ void sel_fetch(float *to, const float *from, int E, i
 //   3. a lower bound of the topk-th largest c: of the largest values of the lanes' shares the topk-th; where that leaves more than 32, bisection
 //   4. the candidates, those not provably below it, get a lane each: rank by comparison with all of them, in 64 bits if two are within the error
 // 8192 rows of 288 experts in 8 groups 13.7 us, one row 3.4; selection one after another, all in 64 bits (select_row_slowly), 62 and 13.
+// STAGED: keys (and biases) are there already, as sel_fetch and sel_pad leave them.
+template <bool STAGED>
 __device__ __forceinline__ void select_row(const float *row, const float *bias, int E, int topk, const SelRule &rule, float *keys, int2 *spot, int *picks,
                                            float *weights, int lane) {
     const unsigned all = 0xffffffffu;
@@ -223,11 +234,10 @@ __device__ __forceinline__ void select_row(const float *row, const float *bias, 
         }
         for (; j < turns; ++j, p += 32, q += 32) *p = f(*p, biased ? *q : 0.f);
     };
-    sel_fetch(keys, row, E, lane);
-    if (!exact) sel_fetch(biases, bias, E, lane);
-    if (lane + 32 * (turns - 1) >= E) {                  // (behind the last expert)
-        keys[lane + 32 * (turns - 1)] = -INFINITY;
-        if (!exact) biases[lane + 32 * (turns - 1)] = -INFINITY;
+    if (!STAGED) {
+        sel_fetch(keys, row, E, lane);
+        if (!exact) sel_fetch(biases, bias, E, lane);
+        sel_pad(keys, E, !exact, lane);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncwarp();

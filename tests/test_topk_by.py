@@ -260,6 +260,49 @@ def test_route_by_is_logits_and_selection(pkg, cuda, rows, H, E, k, rule):
     assert np.array_equal(p2.cpu().numpy(), want_p)
     assert (np.abs(w2.cpu().numpy() - want_w) <= WTOL * np.abs(want_w) + 4 * 2.0 ** -126).all()
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("pdl", [0, 1])
+@pytest.mark.parametrize("rows,H,E,k,biased,rule", [
+    (1, 2048, 64, 4, True, {}), (3, 8, 1, 1, True, {}), (8, 40, 16, 3, False, dict(scores="softmax", scale=1.5)), (9, 264, 17, 8, True, dict(renorm=False)),
+    (16, 2048, 64, 8, True, dict(groups=8, keep_groups=3, group_score="top2")), (7, 4096, 128, 31, True, dict(scores="softmax")),
+    (13, 1000, 100, 5, False, dict(groups=4, keep_groups=2, group_score="top2")), (8, 512, 33, 8, True, dict(groups=3, keep_groups=2)),
+    (16, 136, 129, 4, True, {}), (5, 2048, 127, 6, True, dict(scores="softmax", groups=1))])
+def test_route_by_of_few_rows(pkg, cuda, rows, H, E, k, biased, rule, pdl):
+    """The same for few rows, whose experts share a cluster: bias and activations written by the kernels just in front, ties, rows of NaN and infinities."""
+    import torch
+    gen = torch.Generator(device=cuda).manual_seed(rows + E)
+    x = torch.randn((rows, H + 8), generator=gen, device=cuda).to(torch.bfloat16)[:, :H]
+    wr = (torch.randn((E, H), generator=gen, device=cuda) / H ** 0.5).to(torch.bfloat16)
+    source = torch.randn(E, generator=gen, device=cuda) * 0.1
+    bias = torch.full((E,), 5.0, device=cuda) if biased else None
+    if E > 5:
+        wr[E - 1], wr[2] = wr[0], wr[0]                      # three logits alike
+        source[E - 1], source[2] = source[0], source[0]
+    wide = [torch.full((rows, E), 9.0, device=cuda), torch.full((rows + 1, k + 1), -7, dtype=torch.int32, device=cuda), torch.full((rows + 1, k + 1), -7.0, device=cuda)]
+    out = [wide[0], wide[1][:rows], wide[2][:rows]]
+    fresh = x.clone()
+    if rows > 3:
+        fresh[1], fresh[2, 0], fresh[3, 3] = 0, float("nan"), float("inf")
+    torch.cuda.synchronize()
+    for _ in range(3):
+        x.copy_(fresh)
+        if biased:
+            bias.copy_(source)
+        pkg.route_by(x, wr, *out, bias=bias, pdl=pdl, **rule)
+        if biased:
+            bias.fill_(7.0)
+        x.zero_()
+    x.copy_(fresh)
+    l2 = pkg.linear(x, wr, out_dtype=torch.float32)
+    torch.cuda.synchronize()
+    assert torch.equal(l2.view(torch.int32), out[0].view(torch.int32))
+    r = dict(rule)
+    want_p, want_w = table(l2.cpu().numpy(), source.cpu().numpy() if biased else None, k, keep=r.pop("keep_groups", None), **r)
+    assert np.array_equal(out[1].cpu().numpy(), want_p)
+    assert (np.abs(out[2].cpu().numpy() - want_w) <= WTOL * np.abs(want_w) + 4 * 2.0 ** -126).all()
+    assert (wide[1][rows] == -7).all() and (wide[2][rows] == -7.0).all()          # rows behind the last, left as they were
+
+
 
 def test_refusals(pkg):
     """Bad arguments end in a message, in front of any launch (no GPU needed)."""
