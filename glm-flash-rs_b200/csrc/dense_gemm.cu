@@ -224,7 +224,7 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
             const uint64_t desc0 = t5_desc(smem_u32(ring));
             const uint32_t next = d.bn * 64 >> 4;            // from the first 64 k of the rows to the second
             T5Ring at;
-            uint32_t pc = 0;
+            uint32_t pc = 0, left = stages;
             bool ok = true;
             for (int i = 0; i < items * MATS && ok; ++i)
                 for (int s0 = 0; s0 < d.stages && ok; s0 += d.pass, ++pc) {
@@ -232,17 +232,17 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
                     ok = t5_wait<0>(acc_empty + b, ((pc >> 1) & 1) ^ 1, abort_flag, status, GF_STATUS_MMA_TIMEOUT);
                     t5_fence_after();
                     const int end = min(d.pass, d.stages - s0);
-                    for (int s = 0; s < end; ++s) {
+                    for (int s = 0; s < end; ++s, --left) {
                         ok &= t5_wait<0>(full + at.slot, at.parity, abort_flag, status, GF_STATUS_MMA_TIMEOUT);
                         const uint64_t da = desc0 + at.slot * (slot_bytes >> 4), db = da + (DW_A >> 4);
                         if (t5_elect()) {
 #pragma unroll
                             for (int k = 0; k < DW_K / 16; ++k)
                                 t5_mma<2>(acc, da + 2 * (k & 3) + (k >> 2) * (128 * 128 >> 4), db + 2 * (k & 3) + (k >> 2) * next, idesc, k > 0 ? 1u : s > 0);
-                            t5_commit<2>(done + at.slot);
+                            if (left > depth) t5_commit<2>(done + at.slot);        // (somebody waits for it)
                         }
-                        __syncwarp();
                         at.next(depth);
+                        __syncwarp();
                     }
                     if (t5_elect()) t5_commit<2>(acc_full + b);
                     ok = __all_sync(0xffffffffu, ok);        // (a vote a stage costs the tensor core 90 clocks of each)
@@ -375,15 +375,6 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
                 if (!ok) break;
             }
         }
-        // the arrivals of the last commits have come in before this CTA ends
-        if (warp == 4) {
-            uint32_t slot = stages % depth, parity = stages / depth & 1;               // those of the stage that would come next
-#pragma unroll 1
-            for (uint32_t k = ok ? min(stages, depth) : 0; k; --k) {
-                if (slot == 0) { slot = depth; parity ^= 1; }
-                ok &= t5_wait<200>(done + --slot, parity, abort_flag, status, GF_STATUS_MMA_TIMEOUT);
-            }
-        }
         if (!ok) t5_settle();
     }
     t5_fence_before();
@@ -493,11 +484,11 @@ dense_thin_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
                     for (int k = 0; k < DW_K / 16; ++k)
                         t5_mma<1>(acc + m * d.chains * d.t, da + m * (DW_A >> 4) + 2 * (k & 3) + (k >> 2) * (128 * 128 >> 4), db + 2 * (k & 3) + (k >> 2) * next, idesc,
                                   k > 0 ? 1u : in_chain > 0);
-                t5_commit<1>(done + at.slot);
+                if (it + d.depth < mine) t5_commit<1>(done + at.slot);             // (somebody waits for it)
             }
-            __syncwarp();
             ++in_chain;
             at.next(d.depth);
+            __syncwarp();
         }
         if (t5_elect()) t5_commit<1>(&acc_full);
         ok = __all_sync(0xffffffffu, ok);
