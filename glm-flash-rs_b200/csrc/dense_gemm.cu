@@ -194,16 +194,17 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
             const bool along_n = warp == 3;
             const int box = along_n ? d.bn >> 1 : 128;
             T5Ring at;
-            uint32_t it = 0;                                 // stages that this lane has copied
+            const bool leader = t5_elect();
+            uint32_t turn = 0, it = 0;                       // it: stages that this lane has copied
             bool ok = true;
             for (int i = 0; ok && i < items; ++i, tile.next(d)) {
                 const int y = along_n ? tile.n * d.bn + rank * box : tile.m * 256 + rank * 128;
                 for (int m = 0; m < MATS; ++m) {
                     const CUtensorMap *map = along_n ? &maps.b[m] : &maps.a[m];
 #pragma unroll 1
-                    for (int s = 0; s < d.stages; ++s) {
-                        ok &= t5_wait<200>(done + at.slot, at.parity ^ 1, abort_flag, status, GF_STATUS_TMA_TIMEOUT);
-                        if (t5_elect()) {
+                    for (int s = 0; s < d.stages; ++s, ++turn) {
+                        if (turn >= depth) ok &= t5_wait<200>(done + at.slot, at.parity ^ 1, abort_flag, status, GF_STATUS_TMA_TIMEOUT);
+                        if (leader) {
                             if (ok) {
                                 if (rank == 0) mbar_expect_tx(full + at.slot, 2 * box * DW_K * 2);
                                 const uint32_t bar = full0 + 8 * at.slot;
@@ -224,6 +225,7 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
             const uint64_t desc0 = t5_desc(smem_u32(ring));
             const uint32_t next = d.bn * 64 >> 4;            // from the first 64 k of the rows to the second
             T5Ring at;
+            const bool leader = t5_elect();
             uint32_t pc = 0, left = stages;
             bool ok = true;
             for (int i = 0; i < items * MATS && ok; ++i)
@@ -235,7 +237,7 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
                     for (int s = 0; s < end; ++s, --left) {
                         ok &= t5_wait<0>(full + at.slot, at.parity, abort_flag, status, GF_STATUS_MMA_TIMEOUT);
                         const uint64_t da = desc0 + at.slot * (slot_bytes >> 4), db = da + (DW_A >> 4);
-                        if (t5_elect()) {
+                        if (leader) {
 #pragma unroll
                             for (int k = 0; k < DW_K / 16; ++k)
                                 t5_mma<2>(acc, da + 2 * (k & 3) + (k >> 2) * (128 * 128 >> 4), db + 2 * (k & 3) + (k >> 2) * next, idesc, k > 0 ? 1u : s > 0);
@@ -244,7 +246,7 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
                         at.next(depth);
                         __syncwarp();
                     }
-                    if (t5_elect()) t5_commit<2>(acc_full + b);
+                    if (leader) t5_commit<2>(acc_full + b);
                     ok = __all_sync(0xffffffffu, ok);        // (a vote a stage costs the tensor core 90 clocks of each)
                 }
             if (!ok) t5_settle();
@@ -432,11 +434,12 @@ dense_thin_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
     if (warp == 0 || warp == 2) {                            // (they do not wait for the tensor memory)
         pdl_wait();
         T5Ring at;
+        const bool leader = t5_elect();
         int copied = 0;                                      // stages that this lane has copied
 #pragma unroll 1
         for (int it = 0; it < mine; ++it) {
-            ok &= t5_wait<200>(done + at.slot, at.parity ^ 1, abort_flag, status, GF_STATUS_TMA_TIMEOUT);
-            if (t5_elect()) {
+            if (it >= d.depth) ok &= t5_wait<200>(done + at.slot, at.parity ^ 1, abort_flag, status, GF_STATUS_TMA_TIMEOUT);
+            if (leader) {
                 if (ok) {
                     unsigned char *dst = ring + (size_t)at.slot * bytes;
                     mbar_expect_tx(full + at.slot, warp ? d.t * DW_K * 2 : MATS * DW_A);
@@ -467,6 +470,7 @@ dense_thin_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
         const uint32_t next = d.t * 128 >> 4;
         const int chain = d.chains > 1 ? (mine + d.chains - 1) / d.chains : mine;
         int in_chain = 0;
+        const bool leader = t5_elect();
         uint32_t acc = tmem;
         T5Ring at;
         for (int it = 0; it < mine; ++it) {
@@ -477,7 +481,7 @@ dense_thin_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
                 acc += d.t;
             }
             // (A stage is always multiplied whole, zeros behind K and all: a branch around each product made each take 200 clocks.)
-            if (t5_elect()) {
+            if (leader) {
 #pragma unroll
                 for (int m = 0; m < MATS; ++m)
 #pragma unroll
@@ -490,7 +494,7 @@ dense_thin_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
             at.next(d.depth);
             __syncwarp();
         }
-        if (t5_elect()) t5_commit<1>(&acc_full);
+        if (leader) t5_commit<1>(&acc_full);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) t5_settle();
     } else if (warp >= 4) {
