@@ -660,8 +660,14 @@ int dense_gemm(cudaStream_t s, const DenseArgs &a, bool pdl) {
     if (dense_device(&device)) return -1;
     const int pairs = device->sms / 2, mats = a.w[1] ? 2 : 1, stages = (a.K + DW_K - 1) / DW_K, copies = a.K % 64 ? 2 : 1;
     const bool chain = a.out_type == GLMFLASH_F32 && stages > DW_CHAIN;
-    // Wide: N of a tile and the operand along M, what makes the rounds of tiles over the pairs shortest.  A stage of a round takes 4 clocks for each of
-    // N on the tensor cores (with 256 on all SMs as long as the power limit says), 0.17 us and more for its copies once all pairs copy.
+    // ns of either kernel with any tiles, fitted to 3520 times (17 to 4096 rows, K 504 to 8192, 288 to 8192 outputs): what this takes is on average 2 %
+    // behind the best of them.
+    // Wide: N of a tile and the operand along M.  Rounds of tiles over the pairs: a stage takes its copies' turns, 4 clocks and more for each of N on
+    // the tensor cores, or its bytes once all pairs copy;  the epilogue (whole rows of outputs a lane, exchanged, cost as little only if they can
+    // be stored in 16 bytes) hides behind the next tile's products.
+    const int size = a.out_type == GLMFLASH_F32 ? 4 : 2;
+    const bool vectors = ((uintptr_t)a.out | a.os * size | (int64_t)a.N * size) % 16 == 0;
+    const double halves = copies == 2 ? 1. : 0.;             // (two copies a stage)
     DenseTiles d = {};
     bool rows_m = false;
     d.stages = stages;
@@ -673,12 +679,16 @@ int dense_gemm(cudaStream_t s, const DenseArgs &a, bool pdl) {
             const int64_t tiles = (int64_t)((along + bn - 1) / bn) * across;
             const int64_t rounds = (tiles + pairs - 1) / pairs;
             const double busy = std::min(1., (double)tiles / pairs);
-            const double ns = 4550. + 11. * bn + (double)rounds * mats * (stages * std::max({160., 2.05 * bn, busy * (170. + 1.6 * bn)}) + (chain ? 350. * stages / DW_CHAIN : 0.));
+            const double stage = std::max({256. + 231. * halves, 2.64 * bn, busy * (191. + 1.29 * bn) + 231. * halves});
+            const double body = mats * (stages * stage + (chain ? 350. * stages / DW_CHAIN : 0.)), end = 939. + bn * (!exchanged ? 10.3 : vectors ? 13.3 : 60.);
+            const double ns = 2120. + body + end + (rounds - 1) * std::max(body, end);
             if ((exchanged ? ns < wide : ns <= wide) && tiles <= INT32_MAX / 2) { wide = ns; rows_m = exchanged; d.bn = bn; d.across = across; d.tiles = (int)tiles; }
         }
     }
     GF_REQUIRE(wide < 1e30 && (int64_t)(d.tiles / pairs + 1) * mats * stages < INT32_MAX, "the product is too large");
-    // Thin: rows of a tile and CTAs that cut K.
+    // Thin: rows of a tile and CTAs that cut K.  (Operands beyond what L2 holds at hand: its copies, twice those of pairs, wait for them. 4096 rows, 8192 x
+    // 1024: 74 us, pairs 50.)
+    const double beyond = ((int64_t)a.rows + (int64_t)mats * a.N) * a.K > 24 << 20 ? 0.75 : 0.;
     DenseThin h = {};
     int cluster = 0, row_split = 0;
     double thin = 1e30;
@@ -696,8 +706,9 @@ int dense_gemm(cudaStream_t s, const DenseArgs &a, bool pdl) {
             const int depth = std::min({alias ? (DT_SMEM - 1024) / bytes : apart, most, DT_DEPTH});
             if (depth < std::min(2, most)) continue;
             const double mma = mats * 8 * std::max({41., 33. + 0.25 * t, 0.5 * t}) / 1.9 + 130.;
-            const double ns = 2090. + most * (154. + 0.54 * std::max({mma, bytes / 150., bytes * (double)(across * row_tiles * cn) / 9000.})) +
-                              0.0056 * t * mats * 1024. * (cn - 1) / cn + slots * mats * (88. + 74. * cn);
+            const double work = std::max({mma, bytes / 150., bytes * (double)(across * row_tiles * cn) / 9000.});
+            const double stage = std::max((cn == 1 ? 243. + 0.317 * work : 168. + 0.278 * work) + 185. * halves, beyond * work);
+            const double ns = cn == 1 ? 1257. + most * stage + 24.8 * mats * t : 2150. + most * stage + slots * mats * (78. + 114. * cn);
             if (ns < thin) {
                 thin = ns;
                 cluster = cn;
