@@ -661,7 +661,7 @@ int dense_gemm(cudaStream_t s, const DenseArgs &a, bool pdl) {
     const int pairs = device->sms / 2, mats = a.w[1] ? 2 : 1, stages = (a.K + DW_K - 1) / DW_K, copies = a.K % 64 ? 2 : 1;
     const bool chain = a.out_type == GLMFLASH_F32 && stages > DW_CHAIN;
     // ns of either kernel with any tiles, fitted to 3520 times (17 to 4096 rows, K 504 to 8192, 288 to 8192 outputs): what this takes is on average 2 %
-    // behind the best of them.
+    // behind the best of them.  At the power limit fewer and larger tiles are better (8192 x 4096 x 4096 with N of 256, 224, 192: 208, 214, 222 us).
     // Wide: N of a tile and the operand along M.  Rounds of tiles over the pairs: a stage takes its copies' turns, 4 clocks and more for each of N on
     // the tensor cores, or its bytes once all pairs copy;  the epilogue (whole rows of outputs a lane, exchanged, cost as little only if they can
     // be stored in 16 bytes) hides behind the next tile's products.
@@ -679,7 +679,7 @@ int dense_gemm(cudaStream_t s, const DenseArgs &a, bool pdl) {
             const int64_t tiles = (int64_t)((along + bn - 1) / bn) * across;
             const int64_t rounds = (tiles + pairs - 1) / pairs;
             const double busy = std::min(1., (double)tiles / pairs);
-            const double stage = std::max({256. + 231. * halves, 2.64 * bn, busy * (191. + 1.29 * bn) + 231. * halves});
+            const double stage = std::max({256. + 231. * halves, 60. + 2.4 * bn, busy * (191. + 1.29 * bn) + 231. * halves});
             const double body = mats * (stages * stage + (chain ? 350. * stages / DW_CHAIN : 0.)), end = 939. + bn * (!exchanged ? 10.3 : vectors ? 13.3 : 60.);
             const double ns = 2120. + body + end + (rounds - 1) * std::max(body, end);
             if ((exchanged ? ns < wide : ns <= wide) && tiles <= INT32_MAX / 2) { wide = ns; rows_m = exchanged; d.bn = bn; d.across = across; d.tiles = (int)tiles; }
