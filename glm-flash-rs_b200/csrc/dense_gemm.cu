@@ -9,10 +9,10 @@
 // A tile is one PASS over K into one of two sets of accumulators.  The gated pair is two passes, gate and up, on the same rows; the
 // epilogue keeps act(gate) in registers.  With an fp32 output a pass covers at most 512 k and the epilogue adds passes in fp32 (CHAIN): the
 // tensor core truncates as it accumulates, over 4096 k far beyond what fp32 sums are off by.
-// Stages are 128 k long because a turn of the copying thread (wait, announce, copy) takes 170 ns whatever it copies, and each copy beyond the
-// first 37 (weights and rows have a thread each): with 64 k and two copies a turn an SM took in 80 GB/s, with one CTA alone as with 148, at any
-// depth of the ring; it can take 117 (all SMs at once).  Where K is a multiple of 64 one copy brings both halves of a stage.
-// 8192 x 4096 x 4096 with a residual: 161 us cold at full clocks, the tensor pipe active for 84 % of it; 215 at the power limit.
+// Stages are 128 k long because a turn of a copying warp (wait, announce, copy) takes 300 to 450 clocks whatever it copies, and each copy beyond the
+// first 70 (weights and rows have a warp each): with 64 k and two copies a turn an SM took in 80 GB/s, with one CTA alone as with 148, at any
+// depth of the ring.  Where K is a multiple of 64 one copy brings both halves of a stage.
+// 8192 x 4096 x 4096 with a residual: 208 us at the power limit (1.3 GHz), one call 161 at 1.65 GHz, the tensor pipe active for 84 % of it.
 // Loops that wait have no way out of them but their end (one that depends on a wait costs 70 to 120 clocks a turn: 180 to 230 in place of 113), and
 // whole warps run them, of which an elected lane copies or multiplies.
 // Every wait is bounded; one that gives up sets the status word, every role leaves, copies in flight land, tensor memory is freed.
@@ -70,7 +70,7 @@ __device__ __forceinline__ void dense_act32(const DenseArgs &a, float (&v)[32], 
     }
     dense_act(v, a.act);
 }
-// (Residual and output pass through L2 without pushing operands out: 8192 x 4096 x 4096 with a residual 221 -> 215 us at the power limit.)
+// (Residual and output pass through L2 without pushing operands out: 8192 x 4096 x 4096 with a residual 221 -> 215 us at the power limit, with the tiles of then.)
 // f(i, address of row i) for 32 rows, of which `count` (more than 0) are there: the others stand on the last.  Addresses without a branch between the
 // loads, so that all are on their way at once, and each from its own product where the strides allow it (one from another they are a chain of 800
 // clocks for 32 rows).
@@ -391,8 +391,8 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
 // part, and sends the sums in fours of rows to the CTA of the cluster that finishes them (distributed shared memory, one way, 16 bytes a
 // lane); after a cluster barrier that one adds the parts in ascending order and runs the epilogue.
 //   warps 0, 2 copy weights and rows;  warp 1 allocates tensor memory and issues the products;  warps 4-11 epilogue
-// us, calls one behind another: 17 x 2048 x 1536 4.2, 45 x 4096 x 4096 7.2, gated 200 x 4096 x 512 9.2 (63 MB through L2 for 10 MB of operands: K cut six
-// ways, copies of 120 CTAs), 500 x 2048 x 1536 9.2.
+// us, calls one behind another: 17 x 2048 x 1536 4.1, 45 x 4096 x 4096 7.0, gated 200 x 4096 x 512 8.2 (77 MB through L2 for 10 MB of operands: K cut four
+// ways, 32 rows a tile, copies of 112 CTAs).  Sending the parts with stores that count on a barrier of their receiver, in place of the cluster's barrier: 4.0, -, 9.4.
 constexpr int DT_THREADS = 384, DT_DEPTH = 8, DT_SMEM = 224 * 1024;
 
 struct DenseThin {
