@@ -139,6 +139,16 @@ def test_linear_large(pkg, cuda, rows, K, N):
     plain_case(pkg, cuda, rows, K, N, torch.float16, None, "silu", torch.float16, torch.float16, 8, rows + K + 1)
 
 
+# the residual under the output in pairs' first and later tiles, tiles of few rows without a cut of K, few outputs against the rows
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,K,N", [(700, 1024, 2040), (6000, 520, 1030), (3000, 1024, 304), (1500, 1000, 300), (300, 512, 8192), (4096, 264, 97), (5000, 128, 1)])
+def test_linear_tilings(pkg, cuda, rows, K, N):
+    import torch
+    plain_case(pkg, cuda, rows, K, N, torch.bfloat16, torch.bfloat16, "gelu_tanh", torch.bfloat16, torch.bfloat16, 0, rows + K, inplace=True)
+    plain_case(pkg, cuda, rows, K, N, torch.float16, None, "none", torch.float32, torch.float16, 8, rows + K + 1)
+    gated_case(pkg, cuda, rows, K, N, torch.bfloat16, torch.float32, "silu", 2.0, torch.bfloat16, 0, rows + K + 2)
+
+
 def gated_case(pkg, cuda, rows, K, N, dtype, bias_t, act, limit, out_t, pitch, seed, only_up=False):
     import torch
     gen = torch.Generator(device=cuda).manual_seed(seed)
