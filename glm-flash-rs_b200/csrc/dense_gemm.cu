@@ -228,10 +228,10 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
             const bool leader = t5_elect();
             uint32_t pc = 0, left = stages;
             bool ok = true;
-            for (int i = 0; i < items * MATS && ok; ++i)
-                for (int s0 = 0; s0 < d.stages && ok; s0 += d.pass, ++pc) {
+            for (int i = 0; i < items * MATS; ++i)
+                for (int s0 = 0; s0 < d.stages; s0 += d.pass, ++pc) {
                     const uint32_t b = pc & 1, acc = tmem + b * DW_ROWS;
-                    ok = t5_wait<0>(acc_empty + b, ((pc >> 1) & 1) ^ 1, abort_flag, status, GF_STATUS_MMA_TIMEOUT);
+                    if (pc >= 2) ok &= t5_wait<0>(acc_empty + b, ((pc >> 1) & 1) ^ 1, abort_flag, status, GF_STATUS_MMA_TIMEOUT);
                     t5_fence_after();
                     const int end = min(d.pass, d.stages - s0);
                     for (int s = 0; s < end; ++s, --left) {
@@ -247,7 +247,6 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
                         __syncwarp();
                     }
                     if (leader) t5_commit<2>(acc_full + b);
-                    ok = __all_sync(0xffffffffu, ok);        // (a vote a stage costs the tensor core 90 clocks of each)
                 }
             if (!ok) t5_settle();
         }
