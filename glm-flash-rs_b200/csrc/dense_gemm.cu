@@ -300,7 +300,7 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
                     }
                     // One copy of the code that follows the sums: the four groups of 32 rows take turns in keep[0].  A pair's first tile has a turn more,
                     // of no rows, while it is multiplied: it brings the instructions in, which took longer than they do, and the first residual
-                    // (1000 x 2048 x 1536 10.4 -> 10.1 us; registers do not last for it in a gated pair).
+                    // (1000 x 2048 x 1536 10.4 -> 10.1 us; registers do not last for it in a gated pair, nor with passes added in fp32: 21 us for 17).
 #pragma unroll 1
                     for (int j = EARLY && !i ? -1 : 0; j < turns; ++j) {
                         float v[32];
