@@ -301,9 +301,13 @@ __device__ __forceinline__ void select_row(const float *row, const float *bias, 
         }
         bool in = g < rule.groups && place < rule.keep;
         if (!(exact && !rule.top2)) {
-            const float worst = sel_value(__reduce_min_sync(all, in ? o : 0xffffffffu)), best = sel_value(__reduce_max_sync(all, in || g >= rule.groups ? 0u : o));
-            const float apart = 2.2f * err * (4.f * most + fabsf(worst) + fabsf(best));                  // (two sums of two)
-            const bool open_question = g < rule.groups && !(in ? value > best + apart : value < worst - apart);
+            // Where the value may lie: c of the group's largest and second are off by err (2 most + |c|) each, however much of them cancels in the sum (without a
+            // bias a sum of two scores, off by less).  Infinite terms are what they are; sums beyond the range are compared like infinities, and tie.
+            const float terms = rule.top2 && !exact && per > 1 ? fabsf(first) + fabsf(second) : fabsf(value);
+            const float off = terms < INFINITY ? 1.1f * err * (4.f * most + terms) : 0.f, low = value - off, high = value + off;
+            const float worst = sel_value(__reduce_min_sync(all, in ? sel_ordered(low) : 0xffffffffu)),
+                        best = sel_value(__reduce_max_sync(all, in || g >= rule.groups ? 0u : sel_ordered(high)));
+            const bool open_question = g < rule.groups && !(in ? low > best : high < worst);
             unsigned left = __ballot_sync(all, open_question);
             if (left && sound) {
                 const int places = rule.keep - __popc(__ballot_sync(all, in && !open_question && lane == g * wide));

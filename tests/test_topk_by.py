@@ -350,3 +350,26 @@ def test_refusals_of_the_binding(pkg, cuda):
     for xx, ww in [(x.float(), wr), (x, wr[:63]), (x[:3], wr), (x[:, :56], wr), (x.cpu(), wr), (x, wr[:, ::2])]:
         with pytest.raises(pkg.GlmFlashError):
             pkg.route_by(xx, ww, l, p, w)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scores", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("groups,per,keep", [(2, 2, 1), (8, 2, 3), (3, 5, 1), (8, 8, 4), (8, 36, 4), (32, 32, 5)])
+def test_sums_of_two_that_cancel(pkg, cuda, scores, groups, per, keep):
+    """Biases that open one expert of a group and close the others by finite values: a group's two largest c cancel, and what decides between the
+    sums is far below the last place of their terms in 32 bits."""
+    g = np.random.default_rng(groups * per)
+    E, k = groups * per, min(4, keep * per)
+    opener = g.integers(0, per, groups) + per * np.arange(groups)
+    logits = g.standard_normal((1500, E)).astype(np.float32)
+    if (groups, per) == (2, 2):
+        opener = np.array([0, 2])
+        logits[0] = [0.6270455, -1.6190524, -0.58814746, -0.1600341]
+    for size in (30.0, 1e2, 1e3, 1e4, 1e5, 1e6, 3e38):
+        bias = np.full(E, -size, np.float32)
+        bias[opener] = size
+        for b in (bias, np.where(np.arange(E) // per % 2 == 0, bias, -bias)):        # (and groups that all but one are open in)
+            want_p, want_w = table(logits, b, k, scores, groups, keep, "top2")
+            got_p, got_w = run(pkg, cuda, logits, b, k, scores=scores, groups=groups, keep_groups=keep, group_score="top2")
+            assert np.array_equal(got_p, want_p), (size, int((got_p != want_p).any(1).sum()))
+            assert (np.abs(got_w - want_w) <= WTOL * np.abs(want_w) + 2.0 ** -126).all()
