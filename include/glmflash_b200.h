@@ -308,8 +308,11 @@ int glmflash_route(void *stream, const uint16_t *x, int x_stride, const uint16_t
  *   weight = s * scale, or with renorm s / (sum of the chosen s) * scale, 0 where that sum is 0
  * The order is that of s and c in 64 bits (values that 32 bits cannot tell apart are no tie); weights are computed in fp32 or more.
  * Every row gets topk different ids in 0..experts-1 and finite weights, whatever its logits: a softmax row whose largest logit
- * is +inf shares 1 among its infinities, one without a logit above -inf has scores of 0.  A bias of -inf closes an expert as
- * long as topk others are open.  As in glmflash_topk the last slot names the shared expert (id = experts) with weight 1. */
+ * is +inf shares 1 among its infinities, one without a logit above -inf has scores of 0.  A bias of -inf (or NaN) closes an
+ * expert as long as topk others are open in the groups that stay: a group stays by its value alone, however many of its experts
+ * are closed, and as a sum of two a group with a single open expert has the value -inf like a closed one.  None
+ * is chosen where at least keep_groups groups have max(2, topk / keep_groups rounded up) or more open and the other groups none.
+ * As in glmflash_topk the last slot names the shared expert (id = experts) with weight 1. */
 typedef struct glmflash_topk_rule {
     int32_t scores;        /* GLMFLASH_SCORES_*                                                                */
     int32_t groups;        /* 1..32, divides experts; 1: no groups                                             */

@@ -373,3 +373,22 @@ def test_sums_of_two_that_cancel(pkg, cuda, scores, groups, per, keep):
             got_p, got_w = run(pkg, cuda, logits, b, k, scores=scores, groups=groups, keep_groups=keep, group_score="top2")
             assert np.array_equal(got_p, want_p), (size, int((got_p != want_p).any(1).sum()))
             assert (np.abs(got_w - want_w) <= WTOL * np.abs(want_w) + 2.0 ** -126).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shut", [-np.inf, np.nan])
+@pytest.mark.parametrize("group_score", ["max", "top2"])
+def test_bias_closes_experts_of_groups(pkg, cuda, group_score, shut):
+    """As the formula has it: a group that stays may hold closed experts, which are chosen where it has too few open ones; as a sum of two a group with one
+    open expert counts like a closed one."""
+    logits, _ = make_logits(30, 24, 6)
+    g = np.random.default_rng(8)
+    for open_ in ([0, 1, 2, 12, 13, 14], [5, 6, 18], [7], [1, 8, 15, 22], [], list(range(18))):
+        bias = np.full(24, shut, np.float32)
+        bias[open_] = g.standard_normal(len(open_)).astype(np.float32) * np.float32(0.1)
+        for groups, keep, k in ((2, 1, 4), (4, 1, 2), (4, 2, 8), (4, 3, 3), (12, 5, 6)):
+            for scores in ("sigmoid", "softmax"):
+                want_p, want_w = table(logits, bias, k, scores, groups, keep, group_score)
+                got_p, got_w = run(pkg, cuda, logits, bias, k, scores=scores, groups=groups, keep_groups=keep, group_score=group_score)
+                assert np.array_equal(got_p, want_p), (open_, groups, keep, scores)
+                assert (np.abs(got_w - want_w) <= WTOL * np.abs(want_w) + 2.0 ** -126).all()
