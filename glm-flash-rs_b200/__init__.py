@@ -10,6 +10,7 @@ import ctypes as C
 import functools
 import os
 import struct
+from operator import index as _index
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 SO_PATH = os.environ.get("GLMFLASH_B200_SO") or os.path.join(_HERE, "libglmflash_b200.so")
@@ -592,9 +593,19 @@ def _hot():
 
 
 @functools.lru_cache(maxsize=256)
+def _packed_rule(scores, groups, keep_groups, group_score, renorm, scale):
+    return _RULE.pack(_named(SCORES, scores, "scores"), groups, keep_groups, _named(GROUP_SCORES, group_score, "group_score"), renorm, scale, 0, 0)
+
+
 def _rule(scores, groups, keep_groups, group_score, renorm, scale):
-    return _RULE.pack(_named(SCORES, scores, "scores"), groups, groups if keep_groups is None else keep_groups,
-                      _named(GROUP_SCORES, group_score, "group_score"), int(bool(renorm)), scale, 0, 0)
+    """The rule as the library reads it, kept by its numbers, never by the objects that hold them: a tensor's may change between calls."""
+    try:
+        groups = _index(groups)
+        if type(scale) is not float:
+            scale = scale.__float__()                      # (float() would read text as well)
+        return _packed_rule(scores, groups, groups if keep_groups is None else _index(keep_groups), group_score, 1 if renorm else 0, scale)
+    except (AttributeError, TypeError, ValueError, OverflowError, struct.error) as e:
+        raise GlmFlashError(f"a rule takes names, whole numbers and a finite scale: {e}") from e
 
 
 def _table_refusal(logits, picks, weights, bias, dev):

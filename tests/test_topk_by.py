@@ -392,3 +392,26 @@ def test_bias_closes_experts_of_groups(pkg, cuda, group_score, shut):
                 got_p, got_w = run(pkg, cuda, logits, bias, k, scores=scores, groups=groups, keep_groups=keep, group_score=group_score)
                 assert np.array_equal(got_p, want_p), (open_, groups, keep, scores)
                 assert (np.abs(got_w - want_w) <= WTOL * np.abs(want_w) + 2.0 ** -126).all()
+
+
+@pytest.mark.gpu
+def test_rules_are_read_at_each_call(pkg, cuda):
+    """A rule's numbers may be any objects that stand for one: what they hold at the call counts, not which object it is.  Others end in the
+    library's error."""
+    import torch
+    logits, bias = make_logits(20, 64, 12)
+    ld, bd = torch.from_numpy(logits).to(cuda), torch.from_numpy(bias).to(cuda)
+    picks, weights = torch.empty((20, 5), dtype=torch.int32, device=cuda), torch.empty((20, 5), device=cuda)
+    scale, keep = torch.tensor(2.5), torch.tensor(2)
+    for s, n in ((2.5, 2), (1.25, 3)):
+        scale.fill_(s)
+        keep.fill_(n)
+        pkg.topk_by(ld, picks, weights, bias=bd, groups=np.int64(4), keep_groups=keep, scale=scale)
+        want_p, want_w = table(logits, bias, 4, groups=4, keep=n, scale=s)
+        assert np.array_equal(picks.cpu().numpy(), want_p)
+        assert (np.abs(weights.cpu().numpy() - want_w) <= WTOL * np.abs(want_w) + 4 * 2.0 ** -126).all()
+    pkg.topk_by(ld, picks, weights, groups=2)
+    for kw in (dict(scale=1e39), dict(scale=None), dict(scale="2"), dict(groups=2.0), dict(groups=1 << 40), dict(keep_groups="1"), dict(scores=[]), dict(scores=None),
+               dict(group_score={})):
+        with pytest.raises(pkg.GlmFlashError):
+            pkg.topk_by(ld, picks, weights, **kw)
