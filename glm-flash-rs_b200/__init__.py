@@ -773,9 +773,12 @@ def _dense(x, w, w_up, out, bias, bias_up, act, residual, out_dtype, limit, stre
         bt = both
     if residual is not None:
         rt, rp, rs = _matrix(residual, rows, N, dt, dev, "the residual")
-    if call(get_stream(dev) if stream is None else stream.cuda_stream,
-            _LINEAR.pack(x.data_ptr(), w.data_ptr(), up, bp, bu, rp, out.data_ptr(), xs, ws, us, rs, os_, rows, K, N, code, bt, rt, ot,
-                         ACTS[act] if act in ACTS else _named(ACTS, act, "act"), limit, pdl, 0, 0), _LINEAR.size):
+    try:
+        args = _LINEAR.pack(x.data_ptr(), w.data_ptr(), up, bp, bu, rp, out.data_ptr(), xs, ws, us, rs, os_, rows, K, N, code, bt, rt, ot,
+                            ACTS[act] if act in ACTS else _named(ACTS, act, "act"), limit, pdl, 0, 0)
+    except (TypeError, OverflowError, struct.error) as e:
+        raise GlmFlashError(f"act must be a name and limit a finite number: {e}") from e
+    if call(get_stream(dev) if stream is None else stream.cuda_stream, args, _LINEAR.size):
         _check(-1)
     return out
 

@@ -435,3 +435,12 @@ print('captured')
     env = dict(os.environ)
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, env=env, timeout=300)
     assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.gpu
+def test_arguments_that_are_no_numbers(pkg, cuda):
+    import torch
+    x, w = torch.zeros((4, 64), dtype=torch.bfloat16, device=cuda), torch.zeros((32, 64), dtype=torch.bfloat16, device=cuda)
+    for kw in (dict(limit=1e39), dict(limit=None), dict(limit="1"), dict(act=[]), dict(act=None)):
+        with pytest.raises(pkg.GlmFlashError):
+            pkg.gated_linear(x, w, w, **kw)
