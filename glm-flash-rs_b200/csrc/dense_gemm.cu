@@ -8,7 +8,8 @@
 //   warps 4-11 epilogue: bias, activation, residual or the gated pair, one rounding, while the next pass is multiplied
 // A tile is one PASS over K into one of two sets of accumulators.  The gated pair is two passes, gate and up, on the same rows; the
 // epilogue keeps act(gate) in registers.  With an fp32 output a pass covers at most 512 k and the epilogue adds passes in fp32 (CHAIN): the
-// tensor core truncates as it accumulates, over 4096 k far beyond what fp32 sums are off by.
+// tensor core truncates as it accumulates, over 4096 k far beyond what fp32 sums are off by.  With a 16-bit output a pass covers 8192 k: rows of one sign
+// lose 1e-4 over 16384 and 1.7e-3 over 262144 in one pass, a half step of fp16 is 5e-4.
 // Stages are 128 k long because a turn of a copying warp (wait, announce, copy) takes 300 to 450 clocks whatever it copies, and each copy beyond the
 // first 70 (weights and rows have a warp each): with 64 k and two copies a turn an SM took in 80 GB/s, with one CTA alone as with 148, at any
 // depth of the ring.  Where K is a multiple of 64 one copy brings both halves of a stage.
@@ -29,7 +30,7 @@ __device__ int dense_status_word;
 
 constexpr int DW_K = 128, DW_A = 128 * DW_K * 2;             // k of a stage; bytes of its weights in a CTA
 constexpr int DW_DEPTH = 5, DW_RING = 3 * (DW_A + 256 * 128), DW_THREADS = 384, DW_ROWS = 256;
-constexpr int DW_CHAIN = 512 / DW_K;                         // stages of a pass that is one of several
+constexpr int DW_CHAIN = 512 / DW_K, DW_CHAIN16 = 8192 / DW_K;   // stages of a pass that is one of several, of an fp32 output and of a 16-bit one
 constexpr size_t DW_SMEM = 1024 + DW_RING + 256;
 constexpr int DW_REGS_COPY = 40, DW_REGS_EPI = 232;          // launched with 168 x 384: (40 + 2 x 232) x 128
 static_assert(DW_REGS_COPY + 2 * DW_REGS_EPI <= 3 * 168, "registers");
@@ -258,7 +259,9 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
         // (nobody waits for the last two passes to be read, and an arrival in the other CTA must not come after that one has left)
         const uint32_t all = (uint32_t)items * MATS * (CHAIN ? (d.stages + d.pass - 1) / d.pass : 1);
         constexpr bool EARLY = MATS == 1 && !CHAIN;
-        const int turns = CHAIN || MATS == 2 ? 4 : (cols + 31) >> 5;
+        // (a gated pair in passes keeps sums of up to 64 rows and as many act(gate) where the output has no room for those)
+        const bool parked = CHAIN && MATS == 2 && a.out_type != GLMFLASH_F32;
+        const int turns = parked ? 2 : CHAIN || MATS == 2 ? 4 : (cols + 31) >> 5;
         uint32_t pc = 0;
         bool ok = true;
         float keep[4][32];                                   // gated: act(gate) of this lane's rows;  CHAIN: sums
@@ -347,9 +350,12 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
                             } else if (m == 0) {
                                 dense_act32<2>(a, v, bias);
                             } else {
-                                // (CHAIN: act(gate) waits in its places of the fp32 output)
+                                // (CHAIN: act(gate) waits in its places of the fp32 output, or behind the sums)
                                 float gate[32];
-                                if (CHAIN) load(gate, a.out, c, a.os, GLMFLASH_F32, count);
+                                if (CHAIN && !parked) load(gate, a.out, c, a.os, GLMFLASH_F32, count);
+                                else if (CHAIN)
+#pragma unroll
+                                    for (int i = 0; i < 32; ++i) gate[i] = keep[2][i];
 #pragma unroll
                                 for (int i = 0; i < 32; ++i) {
                                     v[i] += bias;
@@ -357,7 +363,7 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
                                     v[i] *= CHAIN ? gate[i] : keep[0][i];
                                 }
                             }
-                            if (MATS == 1 || m == 1 || CHAIN) {
+                            if (MATS == 1 || m == 1 || (CHAIN && !parked)) {
                                 const int stored = EARLY && j < 0 ? 0 : count;
                                 if (ROWS_M) dense_store_along(v, a.out, place(c, a.os), a.out_type, stored);
                                 else dense_store32(v, a.out, place(c, a.os), a.os, a.out_type, stored);
@@ -369,7 +375,7 @@ dense_wide_kernel(const __grid_constant__ DenseMaps maps, const DenseArgs a, con
                                 keep[0][i] = keep[1][i];
                                 keep[1][i] = keep[2][i];
                                 keep[2][i] = keep[3][i];
-                                if (MATS == 2 && !CHAIN) keep[3][i] = v[i];
+                                if (MATS == 2) keep[3][i] = v[i];
                             }
                     }
                 }
@@ -658,7 +664,8 @@ int dense_gemm(cudaStream_t s, const DenseArgs &a, bool pdl) {
     const DenseDevice *device;
     if (dense_device(&device)) return -1;
     const int pairs = device->sms / 2, mats = a.w[1] ? 2 : 1, stages = (a.K + DW_K - 1) / DW_K, copies = a.K % 64 ? 2 : 1;
-    const bool chain = a.out_type == GLMFLASH_F32 && stages > DW_CHAIN;
+    const int pass = a.out_type == GLMFLASH_F32 ? DW_CHAIN : DW_CHAIN16;
+    const bool chain = stages > pass, parked = chain && mats == 2 && a.out_type != GLMFLASH_F32;
     // ns of either kernel with any tiles, fitted to 3520 times (17 to 4096 rows, K 504 to 8192, 288 to 8192 outputs): what this takes is on average 2 %
     // behind the best of them.  At the power limit fewer and larger tiles are better (8192 x 4096 x 4096 with N of 256, 224, 192: 208, 214, 222 us).
     // Wide: N of a tile and the operand along M.  Rounds of tiles over the pairs: a stage takes its copies' turns, 4 clocks and more for each of N on
@@ -670,16 +677,16 @@ int dense_gemm(cudaStream_t s, const DenseArgs &a, bool pdl) {
     DenseTiles d = {};
     bool rows_m = false;
     d.stages = stages;
-    d.pass = chain ? DW_CHAIN : stages;
+    d.pass = chain ? pass : stages;
     double wide = 1e30;
     for (int exchanged = 0; exchanged < 2; ++exchanged) {
         const int across = ((exchanged ? a.rows : a.N) + 255) / 256, along = exchanged ? a.N : a.rows;
-        for (int bn = 32; bn <= DW_ROWS; bn += 32) {         // (N of a pair's product goes in 32)
+        for (int bn = 32; bn <= (parked ? DW_ROWS / 2 : DW_ROWS); bn += 32) {         // (N of a pair's product goes in 32)
             const int64_t tiles = (int64_t)((along + bn - 1) / bn) * across;
             const int64_t rounds = (tiles + pairs - 1) / pairs;
             const double busy = std::min(1., (double)tiles / pairs);
             const double stage = std::max({256. + 231. * halves, 60. + 2.4 * bn, busy * (191. + 1.29 * bn) + 231. * halves});
-            const double body = mats * (stages * stage + (chain ? 350. * stages / DW_CHAIN : 0.)), end = 939. + bn * (!exchanged ? 10.3 : vectors ? 13.3 : 60.);
+            const double body = mats * (stages * stage + (chain ? 350. * stages / pass : 0.)), end = 939. + bn * (!exchanged ? 10.3 : vectors ? 13.3 : 60.);
             const double ns = 2120. + body + end + (rounds - 1) * std::max(body, end);
             if ((exchanged ? ns < wide : ns <= wide) && tiles <= INT32_MAX / 2) { wide = ns; rows_m = exchanged; d.bn = bn; d.across = across; d.tiles = (int)tiles; }
         }
@@ -697,7 +704,7 @@ int dense_gemm(cudaStream_t s, const DenseArgs &a, bool pdl) {
         if (t > 256 || row_tiles < tiles) continue;
         for (int cn = 1; cn <= 8 && cn <= stages; ++cn) {
             if ((int64_t)across * row_tiles > device->clusters[cn]) continue;
-            const int most = (stages + cn - 1) / cn, chains = chain ? (most + DW_CHAIN - 1) / DW_CHAIN : 1, bytes = mats * DW_A + t * DW_K * 2;
+            const int most = (stages + cn - 1) / cn, chains = chain ? (most + pass - 1) / pass : 1, bytes = mats * DW_A + t * DW_K * 2;
             const int slots = (t / 4 + cn - 1) / cn, parts = cn == 1 ? 0 : cn * slots * mats * 2048, need = mats * chains * t + (t % 32 ? 16 : 0);
             if (need > 512 || parts > DT_SMEM - 1024) continue;
             const int room = DT_SMEM - 1024 - parts, apart = std::min(room / bytes, most);

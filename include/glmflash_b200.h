@@ -341,7 +341,8 @@ int glmflash_route_by(void *stream, const uint16_t *x, int64_t x_stride, const u
  *   w_up == NULL   out = act(x . w^T + bias) + residual
  *   w_up != NULL   out = act(min(g, limit)) * min(max(u, -limit), limit),  g = x . w^T + bias, u = x . w_up^T + bias_up
  * x [rows][x_stride], weights [outer][stride], of `type`; only the first `inner` elements of a row are read.  Sums and the epilogue
- * are fp32, the result is rounded once, to out_type.  residual [rows][residual_stride] may be the output itself (same type and
+ * are fp32, the result is rounded once, to out_type (tensor cores truncate as they accumulate: over at most 512 elements for an fp32
+ * output and 8192 for a 16-bit one, parts longer than that are added in fp32).  residual [rows][residual_stride] may be the output itself (same type and
  * stride); the output may overlap nothing else.  Strides in elements; those of x and the weights multiples of 8, their bases 16-byte
  * aligned; output and residual of any stride.  NaN and infinities go through as the formula says (a limit does not hide a NaN).
  * With an owner whose shared_exl3 is 0 the dense shared expert of a layer is the gated form into a buffer and the plain form

@@ -44,3 +44,93 @@ def test_gelu_of_the_largest_values(pkg, cuda, rows):
     assert torch.equal(torch.isnan(got), torch.isnan(want).expand(rows, -1)) and int(torch.isnan(want).sum()) == 2
     fine = ~torch.isnan(want)
     assert torch.equal(got.double()[:, fine], want[fine].expand(rows, -1).float().double())
+
+
+def aligned(rows, N, dtype, cuda, more):
+    import torch
+    buf = torch.full((rows + 2, N + more), -7.0, dtype=dtype, device=cuda)
+    return buf, buf[:rows, :N]
+
+
+def plain(pkg, cuda, rows, K, N, dtype, bias_t, act, res_t, out_t, seed, res_more=0, inplace=False):
+    """Output rows 16-byte aligned (8 elements of room behind each), residual rows aligned or not."""
+    import torch
+    gen = torch.Generator(device=cuda).manual_seed(seed)
+    x, w = wide(gen, rows, K, -K % 8 + 8, dtype), wide(gen, N, K, -K % 8, dtype, K ** -0.5)
+    bias = None if bias_t is None else torch.randn(N, generator=gen, device=cuda).to(bias_t)
+    buf, out = aligned(rows, N, out_t, cuda, 8)
+    residual = None
+    if res_t is not None:
+        residual = torch.randn((rows, N + res_more), generator=gen, device=cuda).to(res_t)[:, :N]
+        if inplace:
+            out.copy_(residual)
+            residual = out.clone()
+    v = x.double() @ w.double().t()
+    if bias is not None:
+        v = v + bias.double()
+    tol = sum_tol(x, w, bias) * SLOPE + OWN * v.abs()
+    want = act64(v, act)
+    if residual is not None:
+        want = want + residual.double()
+        tol = tol + want.abs() * 2.0 ** -24
+    pkg.linear(x, w, out=out, bias=bias, act=act, residual=out if inplace else residual)
+    torch.cuda.synchronize()
+    check(out, want, tol, out_t)
+    assert untouched(buf, rows, N)
+
+
+def gated(pkg, cuda, rows, K, N, dtype, bias_t, act, limit, out_t, seed):
+    import torch
+    gen = torch.Generator(device=cuda).manual_seed(seed)
+    x = wide(gen, rows, K, -K % 8, dtype)
+    wg, wu = wide(gen, N, K, -K % 8, dtype, 2 * K ** -0.5), wide(gen, N, K, -K % 8 + 8, dtype, 2 * K ** -0.5)
+    bg, bu = (None, None) if bias_t is None else (torch.randn(N, generator=gen, device=cuda).to(bias_t) for _ in range(2))
+    g, u = x.double() @ wg.double().t(), x.double() @ wu.double().t()
+    if bg is not None:
+        g, u = g + bg.double(), u + bu.double()
+    dg, du = sum_tol(x, wg, bg), sum_tol(x, wu, bu)
+    if limit:
+        g, u = g.clamp(max=limit), u.clamp(-limit, limit)
+    a = act64(g, act)
+    tol = (dg * SLOPE + OWN * g.abs()) * (u.abs() + du) + a.abs() * du + (a * u).abs() * 2.0 ** -24
+    buf, out = aligned(rows, N, out_t, cuda, 8)
+    pkg.gated_linear(x, wg, wu, out=out, bias_gate=bg, bias_up=bu, act=act, limit=limit)
+    torch.cuda.synchronize()
+    check(out, a * u, tol, out_t)
+    assert untouched(buf, rows, N)
+
+
+def product64(x, w):
+    """x . w^T in 64 bits, 8192 k at a time."""
+    return sum(x[:, k:k + 8192].double() @ w[:, k:k + 8192].double().t() for k in range(0, x.shape[1], 8192))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,K,N", [(2048, 65536, 512), (4096, 32768, 256), (512, 131072, 256), (30, 262144, 64), (3, 262144, 64)])
+def test_16_bit_outputs_of_very_long_rows(pkg, cuda, rows, K, N):
+    """Rows of one sign: sums of at most 8192 k, evenly spread, lose at most 2 * (1 + .. + 512) / 512 steps of 2^-23; the additions of sums and of parts of
+    K half a step each; then one rounding.  One sum over all of K would lose K / 16 half steps, more than the rounding."""
+    import torch
+    gen = torch.Generator(device=cuda).manual_seed(rows)
+    x = (1 + torch.rand((rows, K), generator=gen, device=cuda)).half()
+    w, up = ((0.25 + torch.rand((N, K), generator=gen, device=cuda) / 4).mul_(4096 / K).half() for _ in range(2))
+    tol = (2 * 515 + 0.5 * (K / 8192 + 16)) * 2.0 ** -23
+    want, u = product64(x, w) / 4096, product64(x, up) / 4096
+    x *= 2.0 ** -12                                           # (exact: x is 1 at least)
+    got, both = pkg.linear(x, w), pkg.gated_linear(x, w, up, act="none")
+    torch.cuda.synchronize()
+    r = half_step(torch.float16)
+    assert ((got.double() - want).abs() <= want * (r + tol)).all(), float(((got.double() - want) / want).mean())
+    assert ((both.double() - want * u).abs() <= want * u * (r + 2 * tol + tol * tol)).all(), float(((both.double() - want * u) / (want * u)).mean())
+
+
+# 16-bit outputs in more than one pass: gated pairs that keep act(gate) beside their sums, remainders of rows, outputs and K
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,K,N", [(3001, 8264, 1000), (8192, 8320, 64), (8190, 8320, 72), (3000, 16500, 304), (2000, 8968, 1500), (200, 8968, 500), (17, 9000, 40)])
+def test_16_bit_outputs_in_passes(pkg, cuda, rows, K, N):
+    import torch
+    b, h, f = torch.bfloat16, torch.float16, torch.float32
+    gated(pkg, cuda, rows, K, N, b, f, "silu", 2.0, b, rows + K)
+    gated(pkg, cuda, rows, K, N, h, None, "gelu", 0.0, h, rows + K + 1)
+    plain(pkg, cuda, rows, K, N, b, f, "none", b, b, rows + K + 2, 0, True)
+    plain(pkg, cuda, rows, K, N, h, None, "gelu_tanh", f, h, rows + K + 3, 3, False)
