@@ -134,3 +134,36 @@ def test_16_bit_outputs_in_passes(pkg, cuda, rows, K, N):
     gated(pkg, cuda, rows, K, N, h, None, "gelu", 0.0, h, rows + K + 1)
     plain(pkg, cuda, rows, K, N, b, f, "none", b, b, rows + K + 2, 0, True)
     plain(pkg, cuda, rows, K, N, h, None, "gelu_tanh", f, h, rows + K + 3, 3, False)
+
+
+# Few outputs against the rows, so that rows lie along M: remainders of rows and outputs, one and several rounds of tiles, short and long K
+FEW = [(20001, 1024, 288), (3000, 1024, 304), (4096, 4096, 288), (8191, 2048, 64), (8192, 2048, 72), (5001, 584, 88), (3001, 1000, 304), (2500, 2048, 296)]
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,K,N", FEW)
+def test_few_outputs(pkg, cuda, rows, K, N):
+    import torch
+    b, h, f = torch.bfloat16, torch.float16, torch.float32
+    for i, (dtype, bias_t, act, res_t, out_t, res_more, inplace) in enumerate([
+            (b, f, "silu", None, b, 0, False), (h, h, "none", h, h, 0, True), (b, b, "gelu_tanh", f, f, 0, True), (h, f, "relu", f, h, 3, False),
+            (b, None, "none", b, f, 1, False), (h, f, "gelu", None, f, 0, False), (b, None, "none", b, b, 8, False)]):
+        plain(pkg, cuda, rows, K, N, dtype, bias_t, act, res_t, out_t, rows + K + i, res_more, inplace)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,K,N", FEW + [(8192, 4096, 384)])
+def test_few_gated_outputs(pkg, cuda, rows, K, N):
+    import torch
+    b, h, f = torch.bfloat16, torch.float16, torch.float32
+    for i, (dtype, bias_t, act, limit, out_t) in enumerate([(b, f, "silu", 10.0, b), (h, None, "gelu_tanh", 0.0, h), (b, b, "silu", 2.0, f), (h, h, "gelu", 0.0, f)]):
+        gated(pkg, cuda, rows, K, N, dtype, bias_t, act, limit, out_t, rows + K + i)
+
+
+# The down projection of a prompt's dense shared expert: fp32 sums of several passes, added to what is there
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,K,N", [(4096, 1536, 2048), (2000, 776, 1500), (3001, 1100, 1001), (1000, 4096, 4096), (300, 2048, 2048), (60, 1536, 2048)])
+def test_long_rows_onto_their_residual(pkg, cuda, rows, K, N):
+    import torch
+    b, h, f = torch.bfloat16, torch.float16, torch.float32
+    plain(pkg, cuda, rows, K, N, b, None, "none", f, f, rows, 0, True)
+    plain(pkg, cuda, rows, K, N, h, f, "silu", h, f, rows + 1, 5, False)
