@@ -167,3 +167,41 @@ def test_long_rows_onto_their_residual(pkg, cuda, rows, K, N):
     b, h, f = torch.bfloat16, torch.float16, torch.float32
     plain(pkg, cuda, rows, K, N, b, None, "none", f, f, rows, 0, True)
     plain(pkg, cuda, rows, K, N, h, f, "silu", h, f, rows + 1, 5, False)
+
+
+def long_tol(x, w, passes=512):
+    """How far a product with an fp32 output may be off.  Sums of at most 512 k: 32 groups of 16, for each at most two truncations by a step of 2^-23 of what has
+    been added up in magnitude so far, the sum of |x w| over the sum's k; that is least tight where all of it comes first, 64 steps of the whole, and on
+    rows whose magnitudes are spread evenly 2 * (1 + .. + 32) / 32 = 33.  Then an fp32 addition for each sum (half a step) and for each of at most 16 parts of K."""
+    K = x.shape[1]
+    groups = math.ceil(min(K, passes) / 16)
+    # evenly spread rows: the first j of n groups hold at most (j + 2) / n of the whole
+    first = 2 * sum(min(1.0, (j + 2) / groups) for j in range(1, groups + 1))
+    return (first + 0.5 * (math.ceil(K / passes) + 16)) * 2.0 ** -23 * (x.double().abs() @ w.double().abs().t())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,K,N", [(1, 4096, 512), (16, 2048, 512), (16, 16384, 520), (40, 16384, 520), (200, 16384, 1000), (2048, 16384, 2048), (4096, 16384, 288), (8192, 8192, 64)])
+def test_fp32_sums_of_long_rows(pkg, cuda, rows, K, N):
+    """fp32 outputs are as far off as sums of 512 k: one sum over all of K, truncated at each step, would lose K / 64 half steps on rows of one sign."""
+    import torch
+    gen = torch.Generator(device=cuda).manual_seed(rows + K)
+    for dtype in (torch.bfloat16, torch.float16):
+        x = (1 + torch.rand((rows, K), generator=gen, device=cuda)).to(dtype)
+        w = (1 + torch.rand((N, K), generator=gen, device=cuda)).to(dtype)
+        want = x.double() @ w.double().t()
+        out, tol = torch.zeros((rows, N), device=cuda), long_tol(x, w)
+        pkg.linear(x, w, out=out)
+        torch.cuda.synchronize()
+        assert ((out - want).abs() <= tol).all(), float(((out - want).abs() / tol).max())
+        up = (torch.rand((N, K), generator=gen, device=cuda) / K).to(dtype)
+        pkg.gated_linear(x, w, up, out=out, act="none")
+        torch.cuda.synchronize()
+        u = x.double() @ up.double().t()
+        both = tol * u + long_tol(x, up) * want + 2 * want * u * 2.0 ** -24
+        assert ((out - want * u).abs() <= both * (1 + 2.0 ** -15)).all(), float(((out - want * u).abs() / both).max())
+        # signs as they come
+        x, w = (torch.randn((n, K), generator=gen, device=cuda).to(dtype) for n in (rows, N))
+        pkg.linear(x, w, out=out)
+        torch.cuda.synchronize()
+        assert ((out - x.double() @ w.double().t()).abs() <= long_tol(x, w)).all()

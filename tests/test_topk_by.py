@@ -415,3 +415,18 @@ def test_rules_are_read_at_each_call(pkg, cuda):
                dict(group_score={})):
         with pytest.raises(pkg.GlmFlashError):
             pkg.topk_by(ld, picks, weights, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,H,E", [(1, 2048, 64), (16, 4096, 128), (9, 4096, 288), (40, 4096, 64), (600, 4096, 288), (4096, 4096, 288), (4096, 8192, 64)])
+def test_logits_of_the_router_in_64_bits(pkg, cuda, rows, H, E):
+    """Ordinary bf16 rows: the logits against the product in 64 bits, by the error of fp32 sums of at most 512 k (test_linear_exact.py has the bound)."""
+    import torch
+    from test_linear_exact import long_tol
+    gen = torch.Generator(device=cuda).manual_seed(rows + H)
+    x = torch.randn((rows, H), generator=gen, device=cuda).to(torch.bfloat16)
+    wr = (torch.randn((E, H), generator=gen, device=cuda) / H ** 0.5).to(torch.bfloat16)
+    logits, picks, weights = torch.empty((rows, E), device=cuda), torch.empty((rows, 5), dtype=torch.int32, device=cuda), torch.empty((rows, 5), device=cuda)
+    pkg.route_by(x, wr, logits, picks, weights)
+    torch.cuda.synchronize()
+    assert ((logits.double() - x.double() @ wr.double().t()).abs() <= long_tol(x, wr)).all()
