@@ -205,3 +205,36 @@ def test_fp32_sums_of_long_rows(pkg, cuda, rows, K, N):
         pkg.linear(x, w, out=out)
         torch.cuda.synchronize()
         assert ((out - x.double() @ w.double().t()).abs() <= long_tol(x, w)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [9, 40, 2000])
+def test_offsets_beyond_32_bits(pkg, cuda, rows):
+    """Rows far apart: offsets of elements past 2^31 and strides past what 32 bits hold for a block of rows."""
+    import torch
+    gen = torch.Generator(device=cuda).manual_seed(rows)
+    K, N, far = 72, 48, (1 << 32) // rows + 8 & -8
+    x = torch.randn((rows, K), generator=gen, device=cuda).to(torch.bfloat16)
+    w, w2 = ((torch.randn((N, K), generator=gen, device=cuda) / 8).to(torch.bfloat16) for _ in range(2))
+    room = torch.empty(rows * far, dtype=torch.bfloat16, device=cuda)
+    fx = room.as_strided((rows, K), (far, 1))
+    fx.copy_(x)
+    fres, out = (room.as_strided((rows, N), (far, 1), room.storage_offset() + 128 + 64 * i) for i in range(2))
+    res = torch.randn((rows, N), generator=gen, device=cuda).to(torch.bfloat16)
+    fres.copy_(res)
+    want, want2 = pkg.linear(x, w, residual=res, act="gelu"), pkg.gated_linear(x, w, w2)
+    pkg.linear(fx, w, residual=fres, act="gelu", out=out)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and torch.equal(fx, x) and torch.equal(fres, res)
+    pkg.linear(fx, w, residual=fres, act="gelu", out=fres)
+    pkg.gated_linear(fx, w, w2, out=out)
+    torch.cuda.synchronize()
+    assert torch.equal(fres, want) and torch.equal(out, want2) and torch.equal(fx, x)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,K,N", [(300000, 64, 8), (300001, 72, 3), (70000, 8, 1)])
+def test_many_rows(pkg, cuda, rows, K, N):
+    import torch
+    plain(pkg, cuda, rows, K, N, torch.bfloat16, torch.float32, "silu", torch.float32, torch.float32, rows, 0, True)
+    gated(pkg, cuda, rows, K, N, torch.float16, None, "silu", 2.0, torch.float16, rows + 1)

@@ -430,3 +430,29 @@ def test_logits_of_the_router_in_64_bits(pkg, cuda, rows, H, E):
     pkg.route_by(x, wr, logits, picks, weights)
     torch.cuda.synchronize()
     assert ((logits.double() - x.double() @ wr.double().t()).abs() <= long_tol(x, wr)).all()
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits(pkg, cuda):
+    """Logits of rows that are far apart, rows of the router product too."""
+    import torch
+    rows, E, far = 20, 96, (1 << 32) // 20
+    logits, bias = make_logits(rows, E, 3)
+    room = torch.empty(rows * far, device=cuda)
+    fl = room.as_strided((rows, E), (far, 1))
+    fl.copy_(torch.from_numpy(logits))
+    picks, weights, b = torch.empty((rows, 5), dtype=torch.int32, device=cuda), torch.empty((rows, 5), device=cuda), torch.from_numpy(bias).to(cuda)
+    pkg.topk_by(fl, picks, weights, bias=b)
+    torch.cuda.synchronize()
+    assert np.array_equal(picks.cpu().numpy(), table(logits, bias, 4)[0])
+    gen = torch.Generator(device=cuda).manual_seed(3)
+    x, wr = torch.randn((rows, 256), generator=gen, device=cuda).to(torch.bfloat16), (torch.randn((E, 256), generator=gen, device=cuda) / 16).to(torch.bfloat16)
+    step = far * 2 // 8 * 8
+    for n in (rows, 7):
+        fx = room.view(torch.bfloat16).as_strided((n, 256), (step, 1))
+        fx.copy_(x[:n])
+        out, want = (([torch.empty((n, E), device=cuda), torch.empty((n, 5), dtype=torch.int32, device=cuda), torch.empty((n, 5), device=cuda)]) for _ in range(2))
+        pkg.route_by(fx, wr, *out, bias=b)
+        pkg.route_by(x[:n], wr, *want, bias=b)
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, want))
