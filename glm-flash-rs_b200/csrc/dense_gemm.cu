@@ -13,7 +13,8 @@
 // Stages are 128 k long because a turn of a copying warp (wait, announce, copy) takes 300 to 450 clocks whatever it copies, and each copy beyond the
 // first 70 (weights and rows have a warp each): with 64 k and two copies a turn an SM took in 80 GB/s, with one CTA alone as with 148, at any
 // depth of the ring.  Where K is a multiple of 64 one copy brings both halves of a stage.
-// 8192 x 4096 x 4096 with a residual: 208 us at the power limit (1.3 GHz), one call 161 at 1.65 GHz, the tensor pipe active for 84 % of it.
+// 8192 x 4096 x 4096 with a residual, calls one behind another: 174 us in the first milliseconds (1.5 GHz and more), 208 to 220 by the GPU once the power limit
+// holds it at 1.3 GHz; the tensor pipe is active for 85 % of the time.
 // Loops that wait have no way out of them but their end (one that depends on a wait costs 70 to 120 clocks a turn: 180 to 230 in place of 113), and
 // whole warps run them, of which an elected lane copies or multiplies.
 // Every wait is bounded; one that gives up sets the status word, every role leaves, copies in flight land, tensor memory is freed.
@@ -667,7 +668,8 @@ int dense_gemm(cudaStream_t s, const DenseArgs &a, bool pdl) {
     const int pass = a.out_type == GLMFLASH_F32 ? DW_CHAIN : DW_CHAIN16;
     const bool chain = stages > pass, parked = chain && mats == 2 && a.out_type != GLMFLASH_F32;
     // ns of either kernel with any tiles, fitted to 3520 times (17 to 4096 rows, K 504 to 8192, 288 to 8192 outputs): what this takes is on average 2 %
-    // behind the best of them.  At the power limit fewer and larger tiles are better (8192 x 4096 x 4096 with N of 256, 224, 192: 208, 214, 222 us).
+    // behind the best of them.  One term is not the fit's: 2.4 clocks and not 2.64 for each of N, so that the larger of two tiles that come out alike is taken, which
+    // at the power limit is the faster one (8192 x 4096 x 4096 with N of 256, 224, 192 on one GPU: 208, 214, 222 us).
     // Wide: N of a tile and the operand along M.  Rounds of tiles over the pairs: a stage takes its copies' turns, 4 clocks and more for each of N on
     // the tensor cores, or its bytes once all pairs copy;  the epilogue (whole rows of outputs a lane, exchanged, cost as little only if they can
     // be stored in 16 bytes) hides behind the next tile's products.

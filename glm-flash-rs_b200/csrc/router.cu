@@ -360,8 +360,8 @@ extern "C" int glmflash_route_by(void *stream, const uint16_t *x, int64_t x_stri
     GF_REQUIRE(x_stride >= hidden && x_stride % 8 == 0, "x_stride must be >= hidden and a multiple of 8");
     GF_REQUIRE(((uintptr_t)x | (uintptr_t)wr) % 16 == 0, "x and the router matrix must be 16-byte aligned");
     GF_REQUIRE(((uintptr_t)logits | (uintptr_t)bias | (uintptr_t)picks | (uintptr_t)weights) % 4 == 0, "logits, bias, picks and weights must be 4-byte aligned");
-    // The dense products, whose kernels are faster than route_kernel for any number of rows and experts (us, logits alone: 2048 x 64 experts, 1 row 2.7
-    // | 3.5, 4096 rows 8.3 | 9.5; 4096 x 288, 1 row 3.7 | 18.4, 4096 rows 18.4 | 72.3), and the selection behind them: in the same
+    // The dense products, whose kernels are faster than route_kernel for any number of rows and experts (us, logits alone: 2048 x 64 experts, 1 row 2.5
+    // | 3.5, 4096 rows 7.3 | 9.3; 4096 x 288, 1 row 3.5 | 18.3, 4096 rows 16.7 | 71.4), and the selection behind them: in the same
     // launch for few rows and experts.
     if (rows <= 16) {
         const DenseArgs few = {x, {wr, nullptr}, {nullptr, nullptr}, nullptr, logits, x_stride, {hidden, 0}, 0, experts, rows, hidden, experts, GLMFLASH_BF16, GLMFLASH_F32, GLMFLASH_F32,

@@ -197,7 +197,7 @@ __device__ __forceinline__ void sel_pad(float *keys, int E, bool biased, int lan
 //   2. groups: 32-bit values by a few lanes a group; those that the error could carry over the border are valued in 64 bits by the whole warp
 //   3. a lower bound of the topk-th largest c: of the largest values of the lanes' shares the topk-th; where that leaves more than 32, bisection
 //   4. the candidates, those not provably below it, get a lane each: rank by comparison with all of them, in 64 bits if two are within the error
-// 8192 rows of 288 experts in 8 groups 13.7 us, one row 3.4; selection one after another, all in 64 bits (select_row_slowly), 62 and 13.
+// 8192 rows of 288 experts in 8 groups 13.5 us, one row 3.4; selection one after another, all in 64 bits (select_row_slowly), 62 and 13.
 // STAGED: keys (and biases) are there already, as sel_fetch and sel_pad leave them.
 template <bool STAGED>
 __device__ __forceinline__ void select_row(const float *row, const float *bias, int E, int topk, const SelRule &rule, float *keys, int2 *spot, int *picks,

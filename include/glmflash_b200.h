@@ -330,7 +330,7 @@ size_t glmflash_topk_rule_bytes(void);
 int glmflash_topk_by(void *stream, const float *logits, int64_t logits_stride, const float *bias, int rows, int experts, int topk,
                      const glmflash_topk_rule *rule, size_t rule_bytes, int32_t *picks, float *weights, int pdl);
 /* The router product and the selection: `logits` (fp32 [rows][experts], caller's) receives the product (the bytes of glmflash_linear
- * with an fp32 output), picks and weights are glmflash_topk_by's of it.  x bf16 [rows][x_stride], wr bf16 [experts][hidden]. */
+ * with an fp32 output of the same place and stride: a product's tiles go by sizes, types and the alignment of its rows), picks and weights are glmflash_topk_by's of it.  x bf16 [rows][x_stride], wr bf16 [experts][hidden]. */
 int glmflash_route_by(void *stream, const uint16_t *x, int64_t x_stride, const uint16_t *wr, const float *bias, int rows, int hidden,
                       int experts, int topk, const glmflash_topk_rule *rule, size_t rule_bytes, float *logits, int32_t *picks,
                       float *weights, int pdl);
